@@ -1,0 +1,542 @@
+// Token-routed experts: the router, the order of the routed rows, and the copies into and out of that order.
+//
+//   eri_expert_route_fwd / _bwd   the k largest scores of a row (ties: the lower index) with softmax weights, and the gradient
+//   eri_expert_plan               stable counting sort of the chosen experts: offsets, row of every choice, choice of every row
+//   eri_expert_scatter            xs[rows[t, j]] = x[t]                      (into expert order)
+//   eri_expert_gather             out[t] = sum_j w[t, j] y[rows[t, j]]       (back; w == nullptr: all ones, the scatter's gradient)
+//   eri_expert_gather_bwd         dy[rows[t, j]] = w[t, j] dout[t], dw[t, j] = <dout[t], y[rows[t, j]]>
+//
+// A choice outside [0, E) (padding) has row -1: it is neither copied nor added, whatever its neighbours hold. Rows from offsets[E]
+// on belong to nobody and are written as zeros. Nothing is added with atomics: every result has one writer and one order of sums.
+#include <limits.h>
+
+#include "ptx.cuh"
+
+using namespace eri;
+typedef __nv_bfloat16 bf16;
+
+namespace {
+
+ERI_DEBUG_BOUNDS_DEFINE(expert_route)
+
+constexpr int kMaxExperts = 1024, kMaxTop = 32;
+
+// e^x for x <= 0 with a relative error near 2^-23: x = n ln2 + r with |r| <= ln2 / 2 (ln2 as the sum of a value of 12 bits,
+// whose product with n is exact, and a rest), Taylor's series of e^r to r^7 (remainder below 2^-27). The special-function unit's
+// 2^x would leave |x| 2^-24 of its argument's rounding in weights that are returned in 32 bits. Below -87: 0.
+__device__ __forceinline__ float exp_nonpos(float x) {
+  if (!(x >= -87.f)) return x != x ? x : 0.f;
+  const float n = rintf(x * 1.4426950408889634f);
+  float r = fmaf(n, -0.693115234375f, x);
+  r = fmaf(n, -3.1946184945309e-05f, r);
+  float p = 1.f / 5040.f;
+  p = fmaf(p, r, 1.f / 720.f);
+  p = fmaf(p, r, 1.f / 120.f);
+  p = fmaf(p, r, 1.f / 24.f);
+  p = fmaf(p, r, 1.f / 6.f);
+  p = fmaf(p, r, 0.5f);
+  p = fmaf(p, r, 1.f);
+  p = fmaf(p, r, 1.f);
+  return __int_as_float(__float_as_int(p) + ((int)n << 23));
+}
+
+// Order of the scores as unsigned integers: -0 equals +0, every NaN is the largest, 0 is no score at all.
+__device__ __forceinline__ uint32_t score_key(float s) {
+  const uint32_t b = __float_as_uint(s);
+  if ((b & 0x7fffffffu) > 0x7f800000u) return 0xffffffffu;
+  if (b == 0x80000000u) return 0x80000000u;
+  return (b >> 31) ? ~b : b | 0x80000000u;
+}
+__device__ __forceinline__ float key_score(uint32_t k) {
+  if (k == 0xffffffffu) return __int_as_float(0x7fffffff);
+  return __uint_as_float((k >> 31) ? k & 0x7fffffffu : ~k);
+}
+
+__device__ __forceinline__ float load_score(const float* s) { return *s; }
+__device__ __forceinline__ float load_score(const bf16* s) { return __bfloat162float(*s); }
+__device__ __forceinline__ void store_score(float* d, float v) { *d = v; }
+__device__ __forceinline__ void store_score(bf16* d, float v) { *d = __float2bfloat16(v); }
+
+constexpr float kNegInf = -__builtin_huge_valf();
+
+// Softmax denominator of a row relative to its largest score m (not -inf): NaN when the row holds a NaN or +inf.
+template <int VPL>
+__device__ __forceinline__ float row_sum(const float (&v)[VPL], float m) {
+  float z = 0.f;
+#pragma unroll
+  for (int i = 0; i < VPL; ++i) z += exp_nonpos(v[i] - m);
+  return warp_sum(z);
+}
+
+// One warp per token; lane l holds the scores of experts l, l + 32, ... in registers. Each of the k rounds is a maximum over the
+// lanes' best keys and a minimum over the indices that reach it (two warp reductions), so equal scores come out in
+// ascending order. Bound by instruction issue for k rounds of VPL + 2 reductions; the scores are read once.
+template <typename T, int VPL>
+__global__ void __launch_bounds__(256) route_fwd_kernel(const T* __restrict__ scores, long long ld, const uint8_t* __restrict__ allowed,
+                                                        long long* __restrict__ idx, float* __restrict__ w, int tokens, int E, int k,
+                                                        int normalize) {
+  const int t = blockIdx.x * 8 + (threadIdx.x >> 5), lane = threadIdx.x & 31;
+  if (t >= tokens) return;
+  const T* s = scores + (long long)t * ld;
+  float v[VPL];
+  uint32_t key[VPL];
+#pragma unroll
+  for (int i = 0; i < VPL; ++i) {
+    const int e = lane + 32 * i;
+    const bool there = e < E;
+    v[i] = there && (!allowed || allowed[e]) ? load_score(s + e) : kNegInf;
+    key[i] = there ? score_key(v[i]) : 0u;
+  }
+  uint32_t my_key = 0u;
+  int my_idx = 0;
+  for (int j = 0; j < k; ++j) {
+    uint32_t best = key[0];
+    int at = 0;
+#pragma unroll
+    for (int i = 1; i < VPL; ++i)
+      if (key[i] > best) {
+        best = key[i];
+        at = i;
+      }
+    const uint32_t top = __reduce_max_sync(0xffffffffu, best);
+    const uint32_t e = __reduce_min_sync(0xffffffffu, best == top ? (uint32_t)(lane + 32 * at) : 0xffffffffu);
+    if (lane == j) {
+      my_key = top;
+      my_idx = (int)e;
+    }
+#pragma unroll
+    for (int i = 0; i < VPL; ++i)
+      if (e == (uint32_t)(lane + 32 * i)) key[i] = 0u;
+  }
+  const float val = key_score(my_key), m = __shfl_sync(0xffffffffu, val, 0);
+  float z = lane < k ? exp_nonpos(val - m) : 0.f, sum;
+  if (m == kNegInf) {              // a row that may choose nothing: no weight
+    z = 0.f;
+    sum = 1.f;
+  } else {
+    sum = normalize ? warp_sum(z) : row_sum<VPL>(v, m);
+  }
+  if (lane < k) {
+    idx[(long long)t * k + lane] = my_idx;
+    w[(long long)t * k + lane] = __fdiv_rn(z, sum);
+  }
+}
+
+// normalize: ds = w_j (dw_j - <w, dw>) at the chosen, zero elsewhere. Otherwise ds = p (g - <w, dw>) with g = dw_j at the chosen.
+template <typename T, int VPL>
+__global__ void __launch_bounds__(256) route_bwd_kernel(const T* __restrict__ scores, long long ld, const uint8_t* __restrict__ allowed,
+                                                        const long long* __restrict__ idx, const float* __restrict__ w,
+                                                        const float* __restrict__ dw, T* __restrict__ ds, int tokens, int E, int k,
+                                                        int normalize) {
+  const int t = blockIdx.x * 8 + (threadIdx.x >> 5), lane = threadIdx.x & 31;
+  if (t >= tokens) return;
+  int my_idx = -1;
+  float wj = 0.f, dj = 0.f;
+  if (lane < k) {
+    my_idx = (int)idx[(long long)t * k + lane];
+    wj = w[(long long)t * k + lane];
+    dj = dw[(long long)t * k + lane];
+  }
+  const float dot = warp_sum(wj * dj);
+  float g[VPL];
+#pragma unroll
+  for (int i = 0; i < VPL; ++i) g[i] = 0.f;
+  const float mine = normalize ? wj * (dj - dot) : dj;
+  for (int j = 0; j < k; ++j) {
+    const int e = __shfl_sync(0xffffffffu, my_idx, j);
+    const float x = __shfl_sync(0xffffffffu, mine, j);
+#pragma unroll
+    for (int i = 0; i < VPL; ++i)
+      if (e == lane + 32 * i) g[i] = x;
+  }
+  if (!normalize) {
+    const T* s = scores + (long long)t * ld;
+    float v[VPL], m = kNegInf;
+    bool nan = false;
+#pragma unroll
+    for (int i = 0; i < VPL; ++i) {
+      const int e = lane + 32 * i;
+      v[i] = e < E && (!allowed || allowed[e]) ? load_score(s + e) : kNegInf;
+      nan |= v[i] != v[i];
+      m = fmaxf(m, v[i]);
+    }
+    m = warp_max(m);
+    if (__any_sync(0xffffffffu, nan)) m = __int_as_float(0x7fffffff);
+    const float sum = m == kNegInf ? 1.f : row_sum<VPL>(v, m);
+#pragma unroll
+    for (int i = 0; i < VPL; ++i) {
+      const float p = m == kNegInf ? 0.f : __fdiv_rn(exp_nonpos(v[i] - m), sum);
+      const bool open = lane + 32 * i < E && (!allowed || allowed[lane + 32 * i]);
+      g[i] = open ? p * (g[i] - dot) : 0.f;
+    }
+  }
+  T* out = ds + (long long)t * E;
+#pragma unroll
+  for (int i = 0; i < VPL; ++i)
+    if (lane + 32 * i < E) store_score(out + lane + 32 * i, g[i]);
+}
+
+// ------------------------------------------------------------------------------------------- plan
+// Stable counting sort by one cluster (one to eight CTAs of 32 warps). Every warp owns a consecutive piece of the choices and a
+// private row of counters in shared memory: (1) it counts its piece, (2) the counters become prefix sums over the warps of a
+// CTA, (3) the CTAs' totals are added over distributed shared memory, (4) the warp walks its piece again and hands out
+// positions. Equal experts inside one group of 32 are ranked by the lanes below, so the order is that of the choices.
+constexpr int kPlanThreads = 1024, kPlanWarps = kPlanThreads / 32;
+
+__device__ __forceinline__ int load_choice(const void* idx, int wide, long long i, int E) {
+  const long long e = wide ? reinterpret_cast<const long long*>(idx)[i] : (long long)reinterpret_cast<const int*>(idx)[i];
+  return e >= 0 && e < E ? (int)e : -1;
+}
+
+__global__ void __launch_bounds__(kPlanThreads) expert_plan_kernel(const void* __restrict__ idx, int wide, int n, int E, int ctas,
+                                                                   int* __restrict__ offsets, int* __restrict__ rows,
+                                                                   int* __restrict__ source) {
+  extern __shared__ int plan_smem[];
+  int* total = plan_smem;                 // [E] this CTA's choices of every expert
+  int* base = total + E;                  // [E] first row of this CTA's choices of every expert
+  int* cnt = base + E;                    // [kPlanWarps][E]
+  __shared__ int s_live;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int rank = ctas > 1 ? (int)cluster_ctarank() : 0;
+  const int warps = ctas * kPlanWarps;
+  const long long piece = (((long long)n + warps - 1) / warps + 31) / 32 * 32;
+  const long long lo = min((long long)(rank * kPlanWarps + warp) * piece, (long long)n), hi = min(lo + piece, (long long)n);
+  int* mine = cnt + (size_t)warp * E;
+  for (int e = lane; e < E; e += 32) mine[e] = 0;
+  __syncwarp();
+  for (long long i0 = lo; i0 < hi; i0 += 128) {       // four loads in flight
+    int c[4];
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+      const long long i = i0 + 32 * u + lane;
+      c[u] = i < hi ? load_choice(idx, wide, i, E) : -1;
+    }
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+      const unsigned same = __match_any_sync(0xffffffffu, c[u]);
+      if (c[u] >= 0 && lane == __ffs(same) - 1) mine[c[u]] += __popc(same);
+      __syncwarp();
+    }
+  }
+  __syncthreads();
+  for (int e = threadIdx.x; e < E; e += kPlanThreads) {
+    int sum = 0;
+    for (int q = 0; q < kPlanWarps; ++q) {
+      const int here = cnt[(size_t)q * E + e];
+      cnt[(size_t)q * E + e] = sum;
+      sum += here;
+    }
+    total[e] = sum;
+  }
+  __syncthreads();
+  if (ctas > 1) cluster_sync_all();
+  // every CTA adds up all totals itself: base[e] = rows of lower experts + rows of e in lower CTAs
+  if (warp == 0) {
+    int run = 0;
+    for (int e0 = 0; e0 < E; e0 += 32) {
+      const int e = e0 + lane;
+      int before = 0, all = 0;
+      if (e < E)
+        for (int c = 0; c < ctas; ++c) {
+          const int x = ctas > 1 ? __float_as_int(ld_shared_cluster_f32(map_to_cta(smem_u32(total + e), (uint32_t)c))) : total[e];
+          all += x;
+          before += c < rank ? x : 0;
+        }
+      int scan = all;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const int up = __shfl_up_sync(0xffffffffu, scan, o);
+        if (lane >= o) scan += up;
+      }
+      if (e < E) {
+        base[e] = run + scan - all + before;
+        if (rank == 0) offsets[e] = run + scan - all;
+      }
+      run += __shfl_sync(0xffffffffu, scan, 31);
+    }
+    if (lane == 0) {
+      s_live = run;
+      if (rank == 0) offsets[E] = run;
+    }
+  }
+  __syncthreads();
+  if (ctas > 1) cluster_sync_all();       // no CTA leaves while another may read its totals
+  for (long long i0 = lo; i0 < hi; i0 += 128) {
+    int c[4];
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+      const long long i = i0 + 32 * u + lane;
+      c[u] = i < hi ? load_choice(idx, wide, i, E) : -1;
+    }
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+      const long long i = i0 + 32 * u + lane;
+      const unsigned same = __match_any_sync(0xffffffffu, c[u]);
+      int pos = -1;
+      if (c[u] >= 0) pos = base[c[u]] + mine[c[u]] + __popc(same & ((1u << lane) - 1u));
+      __syncwarp();
+      if (c[u] >= 0 && lane == __ffs(same) - 1) mine[c[u]] += __popc(same);
+      __syncwarp();
+      if (i < hi) {
+        rows[i] = pos;
+        if (pos >= 0 && ERI_DBG_INDEX(pos, n, 71)) source[pos] = (int)i;
+      }
+    }
+  }
+  for (long long i = (long long)s_live + rank * kPlanThreads + threadIdx.x; i < n; i += (long long)ctas * kPlanThreads) source[i] = -1;
+}
+
+// ------------------------------------------------------------------------------------------- copies
+// A thread owns eight columns of one token. Rows come from the plan; one that is not in [0, n_rows) is skipped.
+__global__ void __launch_bounds__(256) expert_scatter_kernel(const bf16* __restrict__ x, long long ldx, const int* __restrict__ rows,
+                                                             const int* __restrict__ live, bf16* __restrict__ xs, long long items,
+                                                             int vecs, int k, int n_rows, int D) {
+  const long long stride = (long long)gridDim.x * blockDim.x;
+  for (long long it = (long long)blockIdx.x * blockDim.x + threadIdx.x; it < items; it += stride) {
+    const long long t = it / vecs;
+    const int c = (int)(it - t * vecs) * 8;
+    const bf16x8 v = *reinterpret_cast<const bf16x8*>(x + t * ldx + c);
+    for (int j = 0; j < k; ++j) {
+      const int r = rows[t * k + j];
+      if (r >= 0 && r < n_rows) *reinterpret_cast<bf16x8*>(xs + (long long)r * D + c) = v;
+    }
+  }
+  const int from = max(0, min(*live, n_rows));
+  const long long rest = (long long)(n_rows - from) * vecs;
+  bf16x8 z;
+  z.u = make_uint4(0, 0, 0, 0);
+  for (long long it = (long long)blockIdx.x * blockDim.x + threadIdx.x; it < rest; it += stride)
+    *reinterpret_cast<bf16x8*>(xs + (long long)from * D + it * 8) = z;
+}
+
+// out[t] = sum_j w[t, j] y[rows[t, j]] in 32 bits and ascending j, rounded once. Up to four rows of y are in flight per thread.
+__global__ void __launch_bounds__(256) expert_gather_kernel(const bf16* __restrict__ y, long long ldy, const int* __restrict__ rows,
+                                                            const float* __restrict__ w, bf16* __restrict__ out, long long items,
+                                                            int vecs, int k, int n_rows, int D) {
+  const long long stride = (long long)gridDim.x * blockDim.x;
+  for (long long it = (long long)blockIdx.x * blockDim.x + threadIdx.x; it < items; it += stride) {
+    const long long t = it / vecs;
+    const int c = (int)(it - t * vecs) * 8;
+    float acc[8];
+#pragma unroll
+    for (int q = 0; q < 8; ++q) acc[q] = 0.f;
+    for (int j0 = 0; j0 < k; j0 += 4) {
+      bf16x8 v[4];
+      float f[4];
+      bool on[4];
+#pragma unroll
+      for (int u = 0; u < 4; ++u) {
+        const int r = j0 + u < k ? rows[t * k + j0 + u] : -1;
+        on[u] = r >= 0 && r < n_rows;
+        if (on[u]) {
+          v[u] = *reinterpret_cast<const bf16x8*>(y + (long long)r * ldy + c);
+          f[u] = w ? w[t * k + j0 + u] : 1.f;
+        }
+      }
+#pragma unroll
+      for (int u = 0; u < 4; ++u)
+        if (on[u]) {
+          float a[8];
+          unpack8(v[u], a);
+#pragma unroll
+          for (int q = 0; q < 8; ++q) acc[q] = fmaf(f[u], a[q], acc[q]);
+        }
+    }
+    *reinterpret_cast<bf16x8*>(out + t * D + c) = pack8(acc);
+  }
+}
+
+// One CTA per token: dout[t] is read once and meets the token's k rows; the dot products are added in lane and warp order.
+constexpr int kGbThreads = 128, kGbTop = 8;
+__global__ void __launch_bounds__(kGbThreads) expert_gather_bwd_kernel(const bf16* __restrict__ dout, long long ldo,
+                                                                       const bf16* __restrict__ y, long long ldy,
+                                                                       const int* __restrict__ rows, const float* __restrict__ w,
+                                                                       const int* __restrict__ live, bf16* __restrict__ dy,
+                                                                       float* __restrict__ dw, int tokens, int k, int n_rows, int D) {
+  __shared__ float part[kGbThreads / 32][kGbTop];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const long long t = blockIdx.x;
+  if (t < tokens) {
+    for (int j0 = 0; j0 < k; j0 += kGbTop) {
+      float dot[kGbTop], f[kGbTop];
+      int r[kGbTop];
+#pragma unroll
+      for (int u = 0; u < kGbTop; ++u) {
+        dot[u] = 0.f;
+        r[u] = j0 + u < k ? rows[t * k + j0 + u] : -1;
+        if (r[u] >= n_rows) r[u] = -1;
+        f[u] = r[u] >= 0 ? w[t * k + j0 + u] : 0.f;
+      }
+      for (int c = threadIdx.x * 8; c < D; c += kGbThreads * 8) {
+        float g[8];
+        unpack8(*reinterpret_cast<const bf16x8*>(dout + t * ldo + c), g);
+        bf16x8 v[kGbTop];
+        if (dw) {
+#pragma unroll
+          for (int u = 0; u < kGbTop; ++u)
+            if (r[u] >= 0) v[u] = *reinterpret_cast<const bf16x8*>(y + (long long)r[u] * ldy + c);
+        }
+#pragma unroll
+        for (int u = 0; u < kGbTop; ++u)
+          if (r[u] >= 0) {
+            if (dw) {
+              float a[8];
+              unpack8(v[u], a);
+#pragma unroll
+              for (int q = 0; q < 8; ++q) dot[u] = fmaf(g[q], a[q], dot[u]);
+            }
+            if (dy) {
+              float o[8];
+#pragma unroll
+              for (int q = 0; q < 8; ++q) o[q] = f[u] * g[q];
+              *reinterpret_cast<bf16x8*>(dy + (long long)r[u] * D + c) = pack8(o);
+            }
+          }
+      }
+      if (dw) {
+#pragma unroll
+        for (int u = 0; u < kGbTop; ++u) {
+          const float s = warp_sum(dot[u]);
+          if (lane == 0) part[warp][u] = s;
+        }
+        __syncthreads();
+        if (threadIdx.x < kGbTop && j0 + threadIdx.x < k) {
+          float s = 0.f;
+          for (int q = 0; q < kGbThreads / 32; ++q) s += part[q][threadIdx.x];
+          dw[t * k + j0 + threadIdx.x] = s;
+        }
+        __syncthreads();
+      }
+    }
+  }
+  if (dy) {
+    const int from = max(0, min(*live, n_rows));
+    const long long rest = (long long)(n_rows - from) * (D >> 3);
+    bf16x8 z;
+    z.u = make_uint4(0, 0, 0, 0);
+    for (long long it = (long long)blockIdx.x * kGbThreads + threadIdx.x; it < rest; it += (long long)gridDim.x * kGbThreads)
+      *reinterpret_cast<bf16x8*>(dy + (long long)from * D + it * 8) = z;
+  }
+}
+
+template <typename T>
+int route_fwd(const void* s, long long ld, const void* allowed, long long* idx, float* w, int tokens, int E, int k, int normalize,
+              cudaStream_t st) {
+  const unsigned grid = ((unsigned)tokens + 7) / 8;
+#define ERI_ROUTE(V)                                                                                                       \
+  route_fwd_kernel<T, V><<<grid, 256, 0, st>>>((const T*)s, ld, (const uint8_t*)allowed, idx, w, tokens, E, k, normalize)
+  if (E <= 32) ERI_ROUTE(1);
+  else if (E <= 64) ERI_ROUTE(2);
+  else if (E <= 128) ERI_ROUTE(4);
+  else if (E <= 256) ERI_ROUTE(8);
+  else if (E <= 512) ERI_ROUTE(16);
+  else ERI_ROUTE(32);
+#undef ERI_ROUTE
+  return (int)cudaGetLastError();
+}
+
+template <typename T>
+int route_bwd(const void* s, long long ld, const void* allowed, const long long* idx, const float* w, const float* dw, void* ds,
+              int tokens, int E, int k, int normalize, cudaStream_t st) {
+  const unsigned grid = ((unsigned)tokens + 7) / 8;
+#define ERI_ROUTE(V)                                                                                                            \
+  route_bwd_kernel<T, V><<<grid, 256, 0, st>>>((const T*)s, ld, (const uint8_t*)allowed, idx, w, dw, (T*)ds, tokens, E, k, normalize)
+  if (E <= 32) ERI_ROUTE(1);
+  else if (E <= 64) ERI_ROUTE(2);
+  else if (E <= 128) ERI_ROUTE(4);
+  else if (E <= 256) ERI_ROUTE(8);
+  else if (E <= 512) ERI_ROUTE(16);
+  else ERI_ROUTE(32);
+#undef ERI_ROUTE
+  return (int)cudaGetLastError();
+}
+
+// CTAs for `items` threads of work: at most what keeps every SM's 2048 threads busy eight times over, the kernels loop beyond.
+unsigned copy_grid(long long items) {
+  const long long g = (items + 255) / 256;
+  return (unsigned)(g < 1 ? 1 : g > 148 * 64 ? 148 * 64 : g);
+}
+
+bool dims_ok(int tokens, int k, int n_rows, int D) { return tokens >= 1 && k >= 1 && n_rows >= 0 && D >= 8 && D % 8 == 0; }
+
+}  // namespace
+
+extern "C" {
+
+// scores [tokens, E] (row stride ld elements) fp32 (is_bf16 0) or bf16; allowed [E] bytes or null; idx [tokens, k] int64, w fp32.
+int eri_expert_route_fwd(const void* scores, long long ld, const void* allowed, void* idx, float* w, int tokens, int E, int k,
+                         int normalize, int is_bf16, void* stream) {
+  if (tokens < 1 || E < 1 || E > kMaxExperts || k < 1 || k > E || k > kMaxTop || ld < E) return -1;
+  cudaStream_t st = (cudaStream_t)stream;
+  return is_bf16 ? route_fwd<bf16>(scores, ld, allowed, (long long*)idx, w, tokens, E, k, normalize, st)
+                 : route_fwd<float>(scores, ld, allowed, (long long*)idx, w, tokens, E, k, normalize, st);
+}
+
+// ds [tokens, E] contiguous, of the scores' type.
+int eri_expert_route_bwd(const void* scores, long long ld, const void* allowed, const void* idx, const float* w, const float* dw,
+                         void* ds, int tokens, int E, int k, int normalize, int is_bf16, void* stream) {
+  if (tokens < 1 || E < 1 || E > kMaxExperts || k < 1 || k > E || k > kMaxTop || ld < E) return -1;
+  cudaStream_t st = (cudaStream_t)stream;
+  return is_bf16 ? route_bwd<bf16>(scores, ld, allowed, (const long long*)idx, w, dw, ds, tokens, E, k, normalize, st)
+                 : route_bwd<float>(scores, ld, allowed, (const long long*)idx, w, dw, ds, tokens, E, k, normalize, st);
+}
+
+// idx: n choices (int64 when wide, else int32). offsets [E + 1], rows [n], source [n] int32.
+int eri_expert_plan(const void* idx, int wide, int n, int E, int* offsets, int* rows, int* source, void* stream) {
+  if (n < 0 || E < 1 || E > kMaxExperts) return -1;
+  const int smem = (kPlanWarps + 2) * E * (int)sizeof(int);
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return -2;
+  static bool configured[64] = {};
+  if (!configured[dev]) {
+    if (cudaFuncSetAttribute(expert_plan_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                             (kPlanWarps + 2) * kMaxExperts * (int)sizeof(int)) != cudaSuccess)
+      return -3;
+    configured[dev] = true;
+  }
+  // a warp reads 128 choices at a time: more CTAs only when one would loop
+  const int ctas = n <= 4096 ? 1 : n <= 8192 ? 2 : n <= 16384 ? 4 : 8;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(ctas);
+  cfg.blockDim = dim3(kPlanThreads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = (cudaStream_t)stream;
+  cudaLaunchAttribute at[1];
+  at[0].id = cudaLaunchAttributeClusterDimension;
+  at[0].val.clusterDim.x = ctas; at[0].val.clusterDim.y = 1; at[0].val.clusterDim.z = 1;
+  cfg.attrs = at;
+  cfg.numAttrs = ctas > 1 ? 1 : 0;
+  return (int)cudaLaunchKernelEx(&cfg, expert_plan_kernel, idx, wide, n, E, ctas, offsets, rows, source);
+}
+
+// x [tokens, D] (row stride ldx) -> xs [n_rows, D]; live: offsets + E.
+int eri_expert_scatter(const void* x, long long ldx, const int* rows, const int* live, void* xs, int tokens, int k, int n_rows, int D,
+                       void* stream) {
+  if (!dims_ok(tokens, k, n_rows, D) || ldx % 8 || (((uintptr_t)x | (uintptr_t)xs) & 15)) return -1;
+  const long long items = (long long)tokens * (D / 8);
+  expert_scatter_kernel<<<copy_grid(items), 256, 0, (cudaStream_t)stream>>>((const bf16*)x, ldx, rows, live, (bf16*)xs, items, D / 8, k,
+                                                                            n_rows, D);
+  return (int)cudaGetLastError();
+}
+
+int eri_expert_gather(const void* y, long long ldy, const int* rows, const float* w, void* out, int tokens, int k, int n_rows, int D,
+                      void* stream) {
+  if (!dims_ok(tokens, k, n_rows, D) || ldy % 8 || (((uintptr_t)y | (uintptr_t)out) & 15)) return -1;
+  const long long items = (long long)tokens * (D / 8);
+  expert_gather_kernel<<<copy_grid(items), 256, 0, (cudaStream_t)stream>>>((const bf16*)y, ldy, rows, w, (bf16*)out, items, D / 8, k,
+                                                                           n_rows, D);
+  return (int)cudaGetLastError();
+}
+
+// dy [n_rows, D] or null, dw [tokens, k] or null.
+int eri_expert_gather_bwd(const void* dout, long long ldo, const void* y, long long ldy, const int* rows, const float* w, const int* live,
+                          void* dy, float* dw, int tokens, int k, int n_rows, int D, void* stream) {
+  if (!dims_ok(tokens, k, n_rows, D) || ldo % 8 || ldy % 8 || (((uintptr_t)dout | (uintptr_t)y | (uintptr_t)dy) & 15)) return -1;
+  expert_gather_bwd_kernel<<<(unsigned)tokens, kGbThreads, 0, (cudaStream_t)stream>>>((const bf16*)dout, ldo, (const bf16*)y, ldy, rows, w,
+                                                                                       live, (bf16*)dy, dw, tokens, k, n_rows, D);
+  return (int)cudaGetLastError();
+}
+
+}  // extern "C"
+
+ERI_DEBUG_BOUNDS_EXPORT(expert_route)

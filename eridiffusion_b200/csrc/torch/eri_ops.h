@@ -82,6 +82,21 @@ using torch::autograd::variable_list;
                               long long, int, int, int, int, int, int, float, const EriAttnStrides*, void*))     \
   X(eri_flash_attn_wide_fwd, (const void*, const void*, const void*, void*, int, int, int, int, float,           \
                               const EriAttnStrides*, void*))                                                     \
+  X(eri_expert_route_fwd, (const void*, long long, const void*, void*, float*, int, int, int, int, int, void*))  \
+  X(eri_expert_route_bwd, (const void*, long long, const void*, const void*, const float*, const float*, void*,  \
+                           int, int, int, int, int, void*))                                                      \
+  X(eri_expert_plan, (const void*, int, int, int, int*, int*, int*, void*))                                      \
+  X(eri_expert_scatter, (const void*, long long, const int*, const int*, void*, int, int, int, int, void*))      \
+  X(eri_expert_gather, (const void*, long long, const int*, const float*, void*, int, int, int, int, void*))     \
+  X(eri_expert_gather_bwd, (const void*, long long, const void*, long long, const int*, const float*, const int*, \
+                            void*, float*, int, int, int, int, void*))                                           \
+  X(eri_expert_gemm, (int, const void*, long long, const void*, long long, const void*, const int*, void*, int,  \
+                      int, int, int, int, int, long long, void*))                                                \
+  X(eri_linear_4bit, (const void*, long long, const void*, const float*, const int*, const void*, void*, int,    \
+                      int, int, int, int, int, void*))                                                           \
+  X(eri_linear_4bit_planes, (int, int, int))                                                                     \
+  X(eri_linear_4bit_dgrad, (const void*, long long, const void*, const float*, const int*, float*, void*, int,   \
+                            int, int, int, int, int, void*))                                                     \
   X(eri_norm_rope_fwd, (const void*, const void*, long long, const void*, const void*, const float*, const float*, \
                         long long, void*, void*, float*, int, int, int, float, void*))                           \
   X(eri_norm_rope_bwd, (const void*, const void*, long long, const void*, const void*, const float*, const float*, \
@@ -208,6 +223,15 @@ Tensor single_stream(const Tensor& xm, const Tensor& x, const Tensor& gate, cons
                      const Tensor& w2, const OptT& b2, const OptT& a1, const OptT& bb1, double s1, const OptT& a2,
                      const OptT& bb2, double s2, const OptT& qs, const OptT& ks, const OptT& cos, const OptT& sin,
                      int64_t heads, int flags, bool act_fwd_epilogue, bool act_bwd_epilogue);
+
+// ---- expert_ops.cpp
+std::vector<Tensor> expert_route(const Tensor& scores, const OptT& allowed, int64_t k, bool normalize);
+std::vector<Tensor> expert_plan(const Tensor& idx, int64_t experts);
+Tensor expert_dispatch(const Tensor& x, const Tensor& rows, const Tensor& offsets);
+Tensor expert_combine(const Tensor& y, const Tensor& w, const Tensor& rows, const Tensor& offsets);
+Tensor expert_linear(const Tensor& x, const Tensor& w, const Tensor& offsets, int64_t columns, bool accum);
+Tensor linear_4bit(const Tensor& x, const Tensor& codes, const Tensor& scale, const OptT& offsets, const OptT& bias, int64_t experts,
+                   int64_t N, int64_t block, bool nf4);
 
 // Optional tensors among a node's arguments. Function::apply takes them as std::optional, and only the present ones
 // get an edge: ``Args`` records which are present (arguments come first, in order) so that the backward can ask

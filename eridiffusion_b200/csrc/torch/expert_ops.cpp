@@ -1,0 +1,243 @@
+// Token-routed experts and products on 4-bit weights as autograd nodes: router, plan, dispatch, combine, the product grouped by
+// expert and the product on codes. Shapes, types and devices are checked by ops/functional.py; nothing here reads a value back
+// from the device.
+#include "eri_ops.h"
+
+#include <c10/cuda/CUDAGuard.h>
+
+namespace eri_ops {
+
+namespace {
+
+using c10::cuda::CUDAGuard;
+
+// Rows that a kernel reads through a pointer and a row stride (a multiple of 8 elements), copied when they are not laid out so.
+struct Rows {
+  Tensor t;
+  long long ld;
+};
+Rows rows_of(const Tensor& t) {
+  if (rows_ok(t) && t.stride(0) >= t.size(1)) return {t, (long long)t.stride(0)};
+  return {contig16(t), (long long)t.size(1)};
+}
+const int* ints(const Tensor& t) { return t.defined() ? (const int*)t.data_ptr() : nullptr; }
+
+// ------------------------------------------------------------------------------------------- router
+struct ExpertRoute : torch::autograd::Function<ExpertRoute> {
+  static variable_list forward(AutogradContext* ctx, const Tensor& scores, const OptT& allowed_o, int64_t k, bool normalize) {
+    const Tensor allowed = opt(allowed_o);
+    const CUDAGuard guard(scores.device());
+    const Tensor s = scores.stride(1) == 1 && scores.stride(0) >= scores.size(1) ? scores : scores.contiguous();
+    const int64_t T = s.size(0), E = s.size(1);
+    const long long ld = s.is_contiguous() ? E : s.stride(0);
+    Tensor idx = at::empty({T, k}, s.options().dtype(at::kLong)), w = empty_f32({T, k}, s);
+    check(L.eri_expert_route_fwd(s.data_ptr(), ld, ptr(allowed), idx.data_ptr(), (float*)w.data_ptr(), (int)T, (int)E, (int)k, normalize,
+                                 s.scalar_type() == at::kBFloat16, stream()), "expert_route_fwd");
+    if (ctx) {
+      ctx->save_for_backward({s, allowed, idx, w});
+      ctx->saved_data["m"] = std::vector<int64_t>{k, normalize, ld};
+      ctx->mark_non_differentiable({idx});
+      ctx->set_materialize_grads(false);
+    }
+    return {idx, w};
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list gout) {
+    variable_list out(4);
+    if (!gout[1].defined()) return out;
+    auto sv = ctx->get_saved_variables();
+    const Tensor &s = sv[0], &allowed = sv[1], &idx = sv[2], &w = sv[3];
+    const auto m = ctx->saved_data["m"].toIntVector();
+    const CUDAGuard guard(s.device());
+    const Tensor dw = contig(gout[1]);
+    Tensor ds = at::empty({s.size(0), s.size(1)}, s.options());
+    check(L.eri_expert_route_bwd(s.data_ptr(), m[2], ptr(allowed), idx.data_ptr(), (const float*)w.data_ptr(),
+                                 (const float*)dw.data_ptr(), ds.data_ptr(), (int)s.size(0), (int)s.size(1), (int)m[0], (int)m[1],
+                                 s.scalar_type() == at::kBFloat16, stream()), "expert_route_bwd");
+    out[0] = ds;
+    return out;
+  }
+};
+
+// ------------------------------------------------------------------------------------------- dispatch / combine
+Tensor scatter(const Tensor& x_, const Tensor& rows, const Tensor& offsets) {
+  const Rows x = rows_of(x_);
+  const int64_t T = rows.size(0), k = rows.size(1), D = x.t.size(1), E = offsets.size(0) - 1;
+  Tensor xs = empty_bf16({T * k, D}, x.t);
+  check(L.eri_expert_scatter(x.t.data_ptr(), x.ld, ints(rows), ints(offsets) + E, xs.data_ptr(), (int)T, (int)k, (int)(T * k), (int)D,
+                             stream()), "expert_scatter");
+  return xs;
+}
+Tensor gather(const Tensor& y_, const Tensor& rows, const Tensor& w) {
+  const Rows y = rows_of(y_);
+  const int64_t T = rows.size(0), k = rows.size(1), D = y.t.size(1);
+  Tensor out = empty_bf16({T, D}, y.t);
+  check(L.eri_expert_gather(y.t.data_ptr(), y.ld, ints(rows), (const float*)ptr(w), out.data_ptr(), (int)T, (int)k, (int)(T * k), (int)D,
+                            stream()), "expert_gather");
+  return out;
+}
+
+struct ExpertDispatch : torch::autograd::Function<ExpertDispatch> {
+  static Tensor forward(AutogradContext* ctx, const Tensor& x, const Tensor& rows, const Tensor& offsets) {
+    const CUDAGuard guard(x.device());
+    if (ctx) ctx->save_for_backward({rows});
+    return scatter(x, rows, offsets);
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list gout) {
+    const Tensor rows = ctx->get_saved_variables()[0];
+    const CUDAGuard guard(rows.device());
+    return {gather(gout[0], rows, Tensor()), Tensor(), Tensor()};
+  }
+};
+
+struct ExpertCombine : torch::autograd::Function<ExpertCombine> {
+  static Tensor forward(AutogradContext* ctx, const Tensor& y, const Tensor& w_, const Tensor& rows, const Tensor& offsets) {
+    const CUDAGuard guard(y.device());
+    const Tensor w = contig(w_);
+    if (ctx) ctx->save_for_backward({y, w, rows, offsets});
+    return gather(y, rows, w);
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list gout) {
+    auto sv = ctx->get_saved_variables();
+    const Tensor &w = sv[1], &rows = sv[2], &offsets = sv[3];
+    const CUDAGuard guard(rows.device());
+    const Rows y = rows_of(sv[0]), d = rows_of(gout[0]);
+    const int64_t T = rows.size(0), k = rows.size(1), D = y.t.size(1), E = offsets.size(0) - 1;
+    Tensor dy, dw;
+    if (ctx->needs_input_grad(0)) dy = empty_bf16({T * k, D}, y.t);
+    if (ctx->needs_input_grad(1)) dw = empty_f32({T, k}, y.t);
+    if (dy.defined() || dw.defined())
+      check(L.eri_expert_gather_bwd(d.t.data_ptr(), d.ld, y.t.data_ptr(), y.ld, ints(rows), (const float*)w.data_ptr(), ints(offsets) + E,
+                                    mptr(dy), (float*)mptr(dw), (int)T, (int)k, (int)(T * k), (int)D, stream()), "expert_gather_bwd");
+    return {dy, dw, Tensor(), Tensor()};
+  }
+};
+
+// ------------------------------------------------------------------------------------------- grouped product
+enum { kFwd = 0, kDx = 1, kDw = 2 };
+
+struct ExpertLinear : torch::autograd::Function<ExpertLinear> {
+  static Tensor forward(AutogradContext* ctx, const Tensor& x_, const Tensor& w_, const Tensor& offsets, int64_t columns, bool accum) {
+    const CUDAGuard guard(x_.device());
+    const Rows x = rows_of(x_);
+    const Tensor w = contig16(w_);
+    const int64_t R = x.t.size(0), E = w.size(0), N = w.size(1), K = w.size(2);
+    Tensor y = empty_bf16({R, N}, x.t);
+    if (R > 0)
+      check(L.eri_expert_gemm(kFwd, x.t.data_ptr(), x.ld, nullptr, 0, w.data_ptr(), ints(offsets), y.data_ptr(), (int)R, (int)E, (int)N,
+                              (int)K, (int)columns, 0, extent(y), stream()), "expert_gemm");
+    if (ctx) {
+      ctx->save_for_backward({x.t, w, offsets, w_});
+      ctx->saved_data["m"] = std::vector<int64_t>{x.ld, columns, accum};
+    }
+    return y;
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list gout) {
+    auto sv = ctx->get_saved_variables();
+    const Tensor &x = sv[0], &w = sv[1], &offsets = sv[2], &param = sv[3];
+    const auto m = ctx->saved_data["m"].toIntVector();
+    const CUDAGuard guard(x.device());
+    const Rows dy = rows_of(gout[0]);
+    const int64_t R = x.size(0), E = w.size(0), N = w.size(1), K = w.size(2);
+    Tensor dx, dw;
+    if (ctx->needs_input_grad(0)) {
+      dx = empty_bf16({R, K}, x);
+      if (R > 0)
+        check(L.eri_expert_gemm(kDx, dy.t.data_ptr(), dy.ld, nullptr, 0, w.data_ptr(), ints(offsets), dx.data_ptr(), (int)R, (int)E,
+                                (int)N, (int)K, (int)m[1], 0, extent(dx), stream()), "expert_gemm_dx");
+    }
+    if (ctx->needs_input_grad(1)) {
+      const bool acc = has_grad_buffer(param, at::kBFloat16, m[2]) && al16(param.grad());
+      Tensor out = acc ? param.grad() : empty_bf16({E, N, K}, x);
+      if (R > 0)
+        check(L.eri_expert_gemm(kDw, x.data_ptr(), m[0], dy.t.data_ptr(), dy.ld, nullptr, ints(offsets), out.data_ptr(), (int)R, (int)E,
+                                (int)N, (int)K, 0, acc, extent(out), stream()), "expert_gemm_dw");
+      else if (!acc)
+        out.zero_();
+      if (!acc) dw = out;
+    }
+    return {dx, dw, Tensor(), Tensor(), Tensor()};
+  }
+};
+
+// ------------------------------------------------------------------------------------------- 4-bit codes
+struct Linear4bit : torch::autograd::Function<Linear4bit> {
+  static Tensor forward(AutogradContext* ctx, const Tensor& x_, const Tensor& codes, const Tensor& scale, const OptT& offsets_o,
+                        const OptT& bias_o, int64_t E, int64_t N, int64_t block, bool nf4) {
+    const Tensor offsets = opt(offsets_o), bias = opt(bias_o);
+    const CUDAGuard guard(x_.device());
+    const Rows x = rows_of(x_);
+    const int64_t R = x.t.size(0), K = x.t.size(1);
+    Tensor y = empty_bf16({R, N}, x.t);
+    if (R > 0)
+      check(L.eri_linear_4bit(x.t.data_ptr(), x.ld, codes.data_ptr(), (const float*)scale.data_ptr(), ints(offsets), ptr(bias), y.data_ptr(),
+                              (int)R, (int)E, (int)N, (int)K, (int)block, nf4, stream()), "linear_4bit");
+    if (ctx) {
+      ctx->save_for_backward({codes, scale, offsets});
+      ctx->saved_data["m"] = std::vector<int64_t>{R, K, E, N, block, nf4, bias.defined()};
+    }
+    return y;
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list gout) {
+    auto sv = ctx->get_saved_variables();
+    const Tensor &codes = sv[0], &scale = sv[1], &offsets = sv[2];
+    const auto m = ctx->saved_data["m"].toIntVector();
+    const int R = (int)m[0], K = (int)m[1], E = (int)m[2], N = (int)m[3];
+    const CUDAGuard guard(codes.device());
+    Tensor dx, db;
+    if (ctx->needs_input_grad(0)) {
+      const Tensor dy = contig(gout[0]);
+      dx = empty_bf16({R, K}, dy);
+      if (R > 0) {
+        Tensor work = empty_f32({L.eri_linear_4bit_planes(R, N, K), R, K}, dy);
+        check(L.eri_linear_4bit_dgrad(dy.data_ptr(), N, codes.data_ptr(), (const float*)scale.data_ptr(), ints(offsets),
+                                      (float*)work.data_ptr(), dx.data_ptr(), R, E, N, K, (int)m[4], (int)m[5], stream()),
+              "linear_4bit_dgrad");
+      }
+    }
+    // an absent optional argument has no edge; a bias comes without offsets
+    if (m[6] && ctx->needs_input_grad(3)) db = gout[0].sum(0);
+    return {dx, Tensor(), Tensor(), Tensor(), db, Tensor(), Tensor(), Tensor(), Tensor()};
+  }
+};
+
+}  // namespace
+
+std::vector<Tensor> expert_route(const Tensor& scores, const OptT& allowed, int64_t k, bool normalize) {
+  if (any_grad({&scores})) return ExpertRoute::apply(scores, allowed, k, normalize);
+  return ExpertRoute::forward(nullptr, scores, allowed, k, normalize);
+}
+
+std::vector<Tensor> expert_plan(const Tensor& idx_, int64_t experts) {
+  const CUDAGuard guard(idx_.device());
+  const Tensor idx = contig(idx_);
+  const auto o = idx.options().dtype(at::kInt);
+  const int64_t n = idx.numel();
+  Tensor offsets = at::empty({experts + 1}, o), rows = at::empty(idx.sizes(), o), source = at::empty({n}, o);
+  check(L.eri_expert_plan(idx.data_ptr(), idx.scalar_type() == at::kLong, (int)n, (int)experts, (int*)offsets.data_ptr(),
+                          (int*)rows.data_ptr(), (int*)source.data_ptr(), stream()), "expert_plan");
+  return {offsets, rows, source};
+}
+
+Tensor expert_dispatch(const Tensor& x, const Tensor& rows, const Tensor& offsets) {
+  if (any_grad({&x})) return ExpertDispatch::apply(x, rows, offsets);
+  return ExpertDispatch::forward(nullptr, x, rows, offsets);
+}
+
+Tensor expert_combine(const Tensor& y, const Tensor& w, const Tensor& rows, const Tensor& offsets) {
+  if (any_grad({&y, &w})) return ExpertCombine::apply(y, w, rows, offsets);
+  return ExpertCombine::forward(nullptr, y, w, rows, offsets);
+}
+
+Tensor expert_linear(const Tensor& x, const Tensor& w, const Tensor& offsets, int64_t columns, bool accum) {
+  if (any_grad({&x, &w})) return ExpertLinear::apply(x, w, offsets, columns, accum);
+  return ExpertLinear::forward(nullptr, x, w, offsets, columns, accum);
+}
+
+Tensor linear_4bit(const Tensor& x, const Tensor& codes, const Tensor& scale, const OptT& offsets, const OptT& bias_, int64_t experts,
+                   int64_t N, int64_t block, bool nf4) {
+  const Tensor bias = opt(bias_);
+  if (any_grad({&x, &bias})) return Linear4bit::apply(x, codes, scale, offsets, bias_, experts, N, block, nf4);
+  return Linear4bit::forward(nullptr, x, codes, scale, offsets, bias_, experts, N, block, nf4);
+}
+
+}  // namespace eri_ops

@@ -68,7 +68,8 @@ class GatherJob(C.Structure):
 _P, _I, _L, _F, _U64, _U32 = C.c_void_p, C.c_int, C.c_longlong, C.c_float, C.c_ulonglong, C.c_uint
 
 # Kernel families with bounded waits: each has a device error word, read and cleared by eri_<family>_check_error.
-ERROR_FAMILIES = ("gemm", "gemm2", "gemm_few", "gemm_skinny", "gemm_tokred", "fa", "fa2", "fa_wide", "fa_bias", "fa_bwd", "norm")
+ERROR_FAMILIES = ("gemm", "gemm2", "gemm_few", "gemm_skinny", "gemm_tokred", "fa", "fa2", "fa_wide", "fa_bias", "fa_bwd", "norm",
+                  "expert_gemm")
 
 _SIGNATURES = {
     **{f"eri_{f}_check_error": [] for f in ERROR_FAMILIES},
@@ -122,6 +123,16 @@ _SIGNATURES = {
     "eri_gemm2_gather_count": [],
     "eri_rows_wgrad": [_P, _I, _P, _I, _P, _I, _I, _I, _I, _I, _F, _P],
     "eri_rows_dgrad": [_P, _I, _P, _I, _P, _I, _I, _I, _I, _P],
+    "eri_expert_route_fwd": [_P, _L, _P, _P, _P, _I, _I, _I, _I, _I, _P],
+    "eri_expert_route_bwd": [_P, _L, _P, _P, _P, _P, _P, _I, _I, _I, _I, _I, _P],
+    "eri_expert_plan": [_P, _I, _I, _I, _P, _P, _P, _P],
+    "eri_expert_scatter": [_P, _L, _P, _P, _P, _I, _I, _I, _I, _P],
+    "eri_expert_gather": [_P, _L, _P, _P, _P, _I, _I, _I, _I, _P],
+    "eri_expert_gather_bwd": [_P, _L, _P, _L, _P, _P, _P, _P, _P, _I, _I, _I, _I, _P],
+    "eri_expert_gemm": [_I, _P, _L, _P, _L, _P, _P, _P, _I, _I, _I, _I, _I, _I, _L, _P],
+    "eri_linear_4bit": [_P, _L, _P, _P, _P, _P, _P, _I, _I, _I, _I, _I, _I, _P],
+    "eri_linear_4bit_planes": [_I, _I, _I],
+    "eri_linear_4bit_dgrad": [_P, _L, _P, _P, _P, _P, _P, _I, _I, _I, _I, _I, _I, _P],
     "eri_gemv_bf16": [_P, _P, _P, _P, _I, _I, _I, _I, _I, _I, _I, _I, _P],
 }
 
@@ -180,7 +191,7 @@ def debug_bounds_report() -> dict:
     if h is None:
         return out
     buf = (C.c_int * 4)()
-    for tag in ("gemm", "gemm2", "gemm_few", "tokred", "fa", "fa_wide", "fa_bias", "route"):
+    for tag in ("gemm", "gemm2", "gemm_few", "tokred", "fa", "fa_wide", "fa_bias", "route", "expert_route", "expert_gemm"):
         fn = getattr(h, f"eri_{tag}_debug_bounds", None)
         if fn is None:
             if DEBUG_BOUNDS:

@@ -7,6 +7,7 @@ from __future__ import annotations
 
 import math
 import os
+from typing import NamedTuple
 
 import torch
 
@@ -943,3 +944,137 @@ def reinject_rows(full, routed, idx):
     if _native_ok(full, routed) and full.shape[-1] % 8 == 0:
         return _ReinjectRows.apply(full, routed, idx.to(torch.int32).contiguous())
     return full.scatter(1, idx.long().unsqueeze(-1).expand(-1, -1, full.shape[-1]), routed)
+
+
+# ---------------------------------------------------------------------------- token-routed experts
+_MAX_EXPERTS, _MAX_TOP = 1024, 32         # what the router, the plan and the grouped product hold in registers / shared memory
+
+
+class ExpertPlan(NamedTuple):
+    """Order of the routed rows: row r belongs to expert e for ``offsets[e] <= r < offsets[e + 1]`` (int32, on the device);
+    ``rows`` [T, k] is the row of every choice (-1: a choice outside [0, E), e.g. of a padding token), ``source`` [T * k] the
+    choice ``t * k + j`` of every row (-1 from ``offsets[E]`` on)."""
+    offsets: torch.Tensor
+    rows: torch.Tensor
+    source: torch.Tensor
+
+
+def _same_device(what, *ts):
+    devices = {t.device for t in ts if t is not None}
+    if len(devices) > 1:
+        raise ValueError(f"{what}: tensors on different devices: {sorted(str(d) for d in devices)}")
+
+
+def _experts_native(*ts) -> bool:
+    return _BACKEND == "fused" and all(t.is_cuda for t in ts) and N.require() is not None
+
+
+def expert_route(scores, k, allowed=None, normalize=True):
+    """Router of a token: ``scores`` [T, E] -> (expert ids [T, k] int64, weights [T, k] fp32), the ``k`` largest scores in descending
+    order, equal ones by lower index. ``normalize``: the weights are the softmax over the chosen scores (they add up to 1), else
+    the chosen entries of the softmax over the row. ``allowed`` [E] bool: the other experts count as -inf. Weights are
+    differentiable in the scores. A row whose scores are all -inf has weights of zero."""
+    if scores.dim() != 2 or not scores.is_floating_point():
+        raise ValueError(f"expert_route: scores must be [tokens, experts] of a floating type, got {tuple(scores.shape)} {scores.dtype}")
+    T, E = scores.shape
+    if not 1 <= k <= E:
+        raise ValueError(f"expert_route: k = {k} of {E} experts")
+    if allowed is not None:
+        if allowed.dtype != torch.bool or allowed.shape != (E,):
+            raise ValueError(f"expert_route: allowed must be a boolean [{E}], got {tuple(allowed.shape)} {allowed.dtype}")
+        _same_device("expert_route", scores, allowed)
+    if _experts_native(scores) and scores.dtype in (torch.float32, torch.bfloat16) and T > 0 and E <= _MAX_EXPERTS and k <= _MAX_TOP:
+        idx, w = N.ops().expert_route(scores, _c(allowed), k, bool(normalize))
+        return idx, w
+    return R.expert_route(scores, k, allowed, normalize)
+
+
+def expert_plan(idx, num_experts) -> ExpertPlan:
+    """``ExpertPlan`` of the chosen experts ``idx`` [T, k] (int64 or int32): a stable sort by expert, on the device."""
+    if idx.dim() != 2 or idx.dtype not in (torch.int64, torch.int32) or idx.shape[1] < 1:
+        raise ValueError(f"expert_plan: idx must be [tokens, k] int64 or int32, got {tuple(idx.shape)} {idx.dtype}")
+    if num_experts < 1 or idx.numel() >= 2 ** 31:
+        raise ValueError(f"expert_plan: {num_experts} experts, {idx.numel()} choices")
+    if _experts_native(idx) and num_experts <= _MAX_EXPERTS:
+        return ExpertPlan(*N.ops().expert_plan(idx, num_experts))
+    return ExpertPlan(*R.expert_plan(idx, num_experts))
+
+
+def expert_dispatch(x, plan: ExpertPlan):
+    """Tokens ``x`` [T, D] into expert order: [T * k, D], zeros from ``plan.offsets[E]`` on."""
+    T, k = plan.rows.shape
+    if x.dim() != 2 or x.shape[0] != T:
+        raise ValueError(f"expert_dispatch: x {tuple(x.shape)} for a plan of {T} tokens")
+    _same_device("expert_dispatch", x, plan.rows)
+    if _native_ok(x) and x.shape[1] % 8 == 0 and x.numel() > 0:
+        return N.ops().expert_dispatch(x, plan.rows, plan.offsets)
+    return R.expert_dispatch(x, plan.source, k)
+
+
+def expert_combine(y, weights, plan: ExpertPlan):
+    """``out[t] = sum_j weights[t, j] * y[rows[t, j]]``: rows ``y`` [T * k, D] in expert order back to the tokens [T, D]."""
+    T, k = plan.rows.shape
+    if y.dim() != 2 or y.shape[0] != T * k or tuple(weights.shape) != (T, k):
+        raise ValueError(f"expert_combine: y {tuple(y.shape)}, weights {tuple(weights.shape)} for a plan of {T} tokens and {k} choices")
+    _same_device("expert_combine", y, weights, plan.rows)
+    if _native_ok(y) and y.shape[1] % 8 == 0 and y.numel() > 0:
+        return N.ops().expert_combine(y, weights.float(), plan.rows, plan.offsets)
+    return R.expert_combine(y, weights, plan.rows)
+
+
+def _check_offsets(what, offsets, E, x):
+    if offsets.dim() != 1 or offsets.shape[0] != E + 1 or offsets.dtype not in (torch.int32, torch.int64):
+        raise ValueError(f"{what}: offsets must be [{E + 1}] int32 or int64, got {tuple(offsets.shape)} {offsets.dtype}")
+    _same_device(what, x, offsets)
+
+
+def expert_linear(x, w, offsets):
+    """Product grouped by expert: ``y[r] = x[r] @ w[e]^T`` for ``offsets[e] <= r < offsets[e + 1]``; x [R, K] in expert order, w
+    [E, N, K], offsets [E + 1] ascending, on the device (``ExpertPlan.offsets``). Rows of no expert are zeros and get no gradient.
+    Differentiable in x and w; nothing is read back to the host."""
+    if x.dim() != 2 or w.dim() != 3 or x.shape[1] != w.shape[2] or w.shape[0] < 1:
+        raise ValueError(f"expert_linear: x {tuple(x.shape)} and w {tuple(w.shape)} must be [R, K] and [E, N, K]")
+    _check_offsets("expert_linear", offsets, w.shape[0], x)
+    _same_device("expert_linear", x, w)
+    if x.dtype != w.dtype:
+        raise ValueError(f"expert_linear: x {x.dtype}, w {w.dtype}")
+    E, Nn, K = w.shape
+    if _native_ok(x, w) and E <= _MAX_EXPERTS and Nn % 8 == 0 and K % 8 == 0 and Nn > 0 and K > 0 and x.shape[0] < 2 ** 31:
+        return N.ops().expert_linear(x, w, offsets.to(torch.int32).contiguous(), 0, _ACCUM_INTO_GRAD)
+    return R.expert_linear(x, w, offsets)
+
+
+# Most rows that are multiplied with the codes themselves; above, the weight is expanded once and meets the matrix kernels.
+_CODES_ROWS, _CODES_EXPERT_ROWS = 8, 64
+
+
+def linear_4bit(x, q, offsets=None, bias=None):
+    """``x @ W^T (+ bias)`` with a weight stored as int4 or NF4 codes (``memory.QuantizedTensor`` ``q``). ``q.shape`` [N, K]: x
+    [..., K]. ``q.shape`` [E, N, K] with ``offsets`` [E + 1]: x [R, K] in expert order, as in ``expert_linear``. A few bf16 rows
+    on the GPU are multiplied with the codes (the weight in full precision ``level * scale``); more rows expand the weight to bf16
+    first. Differentiable in x and bias."""
+    if q.kind not in ("int4", "nf4"):
+        raise ValueError(f"linear_4bit: {q.kind} weights")
+    experts = len(q.shape) == 3
+    if len(q.shape) not in (2, 3) or experts != (offsets is not None):
+        raise ValueError(f"linear_4bit: a weight of shape {tuple(q.shape)} {'needs' if experts else 'takes no'} offsets")
+    E, (Nn, K) = (q.shape[0] if experts else 1), q.shape[-2:]
+    if x.shape[-1:] != (K,) or (experts and x.dim() != 2):
+        raise ValueError(f"linear_4bit: x {tuple(x.shape)} for a weight of shape {tuple(q.shape)}")
+    if experts:
+        _check_offsets("linear_4bit", offsets, E, x)
+        if bias is not None:
+            raise ValueError("linear_4bit: no bias with offsets")
+    elif bias is not None and tuple(bias.shape) != (Nn,):
+        raise ValueError(f"linear_4bit: bias {tuple(bias.shape)} for {Nn} outputs")
+    _same_device("linear_4bit", x, q.data, q.scale, bias)
+    rows = x.numel() // K
+    if _native_ok(x, bias) and rows <= (_CODES_EXPERT_ROWS if experts else _CODES_ROWS) and K % q.block == 0 and q.block % 32 == 0 \
+            and q.data.is_contiguous() and q.data.data_ptr() % 16 == 0 and Nn > 0:
+        y = N.ops().linear_4bit(x.reshape(rows, K), q.data, q.scale.float().contiguous(),
+                                None if offsets is None else offsets.to(torch.int32).contiguous(), bias, E, Nn, q.block, q.kind == "nf4")
+        return y.view(*x.shape[:-1], Nn)
+    if _native_ok(x):
+        w = q.dequantize(torch.bfloat16)
+        return expert_linear(x, w, offsets) if experts else linear(x, w, bias)
+    return R.linear_4bit(x, q.dequantize(torch.float32), offsets, bias)

@@ -218,3 +218,69 @@ def group_norm_silu(x, weight, bias=None, groups=32, eps=1e-5, silu=True):
     if silu:
         y = torch.nn.functional.silu(y)
     return y.transpose(1, 2).to(x.dtype)
+
+
+# ---------------------------------------------------------------------------- token-routed experts
+def expert_route(scores, k, allowed=None, normalize=True):
+    """The ``k`` largest scores of every row, descending, equal ones in ascending order of index (NaN counts as the
+    largest), and their softmax weights in fp32. A row without any finite score has weights of zero."""
+    s = scores.float()
+    if allowed is not None:
+        s = torch.where(allowed, s, float("-inf"))
+    idx = torch.sort(s.detach(), dim=-1, descending=True, stable=True).indices[:, :k]
+    top = s.gather(1, idx)
+    m = top.detach()[:, :1]
+    m = torch.where(m == float("-inf"), 0.0, m)
+    z = torch.exp(top - m)
+    total = (z if normalize else torch.exp(s - m)).sum(-1, keepdim=True)
+    return idx.contiguous(), z / torch.where(total == 0, 1.0, total)
+
+
+def expert_plan(idx, num_experts):
+    """(offsets [E + 1], rows [T, k], source [T * k]) int32 of the stable sort of the choices by expert."""
+    flat = idx.reshape(-1).long()
+    valid = (flat >= 0) & (flat < num_experts)
+    key = torch.where(valid, flat, num_experts)
+    order = torch.sort(key, stable=True).indices
+    counts = torch.zeros(num_experts + 1, dtype=torch.int64, device=idx.device).index_add_(0, key, torch.ones_like(key))
+    offsets = torch.cat([counts.new_zeros(1), counts[:num_experts].cumsum(0)])
+    place = torch.arange(flat.numel(), device=idx.device)
+    rows = torch.empty_like(order)
+    rows[order] = place
+    rows = torch.where(valid, rows, -1).view(idx.shape)
+    return offsets.int(), rows.int(), torch.where(place < offsets[-1], order, -1).int()
+
+
+def expert_dispatch(x, source, k):
+    token = torch.div(source.clamp_min(0).long(), k, rounding_mode="floor")
+    return torch.where((source >= 0)[:, None], x.float()[token], 0.0).to(x.dtype)
+
+
+def expert_combine(y, w, rows):
+    yt = torch.where((rows >= 0)[..., None], y.float()[rows.clamp_min(0).long()], 0.0)
+    return (w.float()[..., None] * yt).sum(1).to(y.dtype)
+
+
+def _segments(offsets, rows):
+    """Bounds of the experts' rows on the host, ascending inside [0, rows]."""
+    out, low = [], 0
+    for o in offsets.tolist():
+        low = max(low, min(o, rows))
+        out.append(low)
+    return out
+
+
+def expert_linear(x, w, offsets):
+    b = _segments(offsets, x.shape[0])
+    xf = x.float()
+    parts = [xf[b[e]:b[e + 1]] @ w[e].float().t() for e in range(w.shape[0])]
+    n = w.shape[1]
+    return torch.cat([xf.new_zeros(b[0], n), *parts, xf.new_zeros(x.shape[0] - b[-1], n)]).to(x.dtype)
+
+
+def linear_4bit(x, weight, offsets=None, bias=None):
+    """``weight``: the expanded fp32 weight, [N, K] or [E, N, K]."""
+    if offsets is not None:
+        return expert_linear(x, weight, offsets)
+    y = x.float() @ weight.t()
+    return (y if bias is None else y + bias.float()).to(x.dtype)
