@@ -5,7 +5,9 @@
 //   eri_linear_4bit_dgrad  dx[r, k] = sum_n dy[r, n] level(q[e, n, k]) scale[e, n, k / block]
 //
 // e: the expert of row r, offsets[e] <= r < offsets[e + 1] (offsets null: one weight for all rows). Rows of no expert are zeros. A CTA
-// takes up to kRows rows of one expert; the CTA of any other row of theirs leaves at once.
+// takes up to eight rows of one expert; the CTA of any other row of theirs leaves at once.
+#include <cuda_fp16.h>
+
 #include "ptx.cuh"
 
 using namespace eri;
@@ -26,8 +28,8 @@ struct Segment {
   int e, rows;        // rows of this CTA from row r on: 0 = another CTA's, -1 = row r belongs to no expert
 };
 // offsets ascend; whatever they hold, the rows stay in [0, R).
-__device__ __forceinline__ Segment segment_of(const int* offsets, int E, int R, int r) {
-  if (!offsets) return Segment{0, r % kRows == 0 ? min(kRows, R - r) : 0};
+__device__ __forceinline__ Segment segment_of(const int* offsets, int E, int R, int r, int most) {
+  if (!offsets) return Segment{0, r % most == 0 ? min(most, R - r) : 0};
   int lo = 0, hi = E + 1;                // the last e with offsets[e] <= r, plus one
   while (lo < hi) {
     const int mid = (lo + hi) >> 1;
@@ -37,47 +39,283 @@ __device__ __forceinline__ Segment segment_of(const int* offsets, int E, int R, 
   if (e < 0 || e >= E) return Segment{0, -1};
   const int first = max(0, offsets[e]), end = min(R, offsets[e + 1]);
   if (r < first || r >= end) return Segment{0, -1};
-  return Segment{e, (r - first) % kRows == 0 ? min(kRows, end - r) : 0};
+  return Segment{e, (r - first) % most == 0 ? min(most, end - r) : 0};
 }
 
-__global__ void __launch_bounds__(256) linear_4bit_kernel(const bf16* __restrict__ x, long long ldx, const uint8_t* __restrict__ codes,
-                                                          const float* __restrict__ scale, const int* __restrict__ offsets,
-                                                          const bf16* __restrict__ bias, bf16* __restrict__ y, int R, int E, int N, int K, int block, int nf4) {
-  const int r0 = blockIdx.y;
-  const Segment sg = segment_of(offsets, E, R, r0);
-  const int n = blockIdx.x * 8 + (threadIdx.x >> 5), lane = threadIdx.x & 31;
-  __shared__ float lv[16];
-  if (threadIdx.x < 16) lv[threadIdx.x] = c_level[nf4][threadIdx.x];
-  __syncthreads();
-  if (sg.rows == 0 || n >= N) return;
+// ------------------------------------------------------------------------------------------- y = x W^T
+// Sixteen weight rows are the rows of A in mma.m16n8k16, up to eight rows of x its columns. A lane decodes a quarter of a step of one
+// weight row and of the row eight below it (8 or 16 codes each; the order of the reduction inside a step is free, so x is laid
+// out in the order in which the codes come out of a word). The products of a step have one scale per weight row, which
+// multiplies their fp32 sum; nothing is expanded in memory.
+//   int4   code - 8 as bf16 (exact), x as it is: the products are exact; the seventh of the level multiplies the finished sum.
+//   NF4    levels as fp16 (2^-12), fetched two at a time from a table of all 256 bytes in shared memory that every lane has for itself
+//          (a bank of its own, so no conflicts). x as fp16 times a power of two that brings its largest magnitude in the step to
+//          [2^14, 2^15): values down to 2^-32 of that are exact, the rest is off by 2^-39 of it.
+// The reduction is split over the `kw` warps of a group, `nw` groups take 16 weight rows each. A warp copies the pieces of codes that
+// it alone reads (four steps of 16 rows) asynchronously into a ring of its own, across the tiles of a persistent CTA, so that no
+// warp waits for another but for the sum of a tile: partial sums meet in shared memory and are added in warp order.
+constexpr int kU = 4;                       // steps of a piece
+constexpr int kMaxWarps = 20;
+constexpr int kTable = 256 * 32 * 4;        // bytes of the NF4 table
+constexpr int kRedRow = 20;                 // partial sums: [warp][8 columns][16 rows + 4], so that a warp's stores hit 32 banks
+
+__device__ __forceinline__ uint32_t half2_bits(float a, float b) {
+  const __half2 h = __floats2half2_rn(a, b);
+  return *reinterpret_cast<const uint32_t*>(&h);
+}
+__device__ __forceinline__ void copy16(uint32_t dst, const void* src) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+}
+__device__ __forceinline__ void copy4(uint32_t dst, const void* src) {
+  asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(dst), "l"(src) : "memory");
+}
+__device__ __forceinline__ void copy_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void copy_wait() {
+  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+}
+// d += A B
+template <bool NF4>
+__device__ __forceinline__ void mma16816(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+  if constexpr (NF4)
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+        : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+  else
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+        : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+// Eight codes of a word as four pairs: int4 (0,4) (1,5) (2,6) (3,7), NF4 (0,1) (2,3) (4,5) (6,7).
+template <bool NF4>
+__device__ __forceinline__ void decode8(uint32_t c, const uint8_t (&table)[NF4 ? kTable : 16], uint32_t lane4, uint32_t (&h)[4]) {
+  if constexpr (NF4) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      h[i] = *reinterpret_cast<const uint32_t*>(table + (((i == 0 ? c << 7 : c >> (8 * i - 7)) & 0x7f80u) | lane4));
+  } else {
+    const __nv_bfloat162 off = __floats2bfloat162_rn(136.f, 136.f);       // 128 + code - 136, exact
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      uint32_t v = ((c >> (4 * i)) & 0x000f000fu) | 0x43004300u;
+      const __nv_bfloat162 w = __hsub2(*reinterpret_cast<__nv_bfloat162*>(&v), off);
+      h[i] = *reinterpret_cast<const uint32_t*>(&w);
+    }
+  }
+}
+
+struct Args4 {
+  const bf16* x;
+  long long ldx;
+  const uint8_t* codes;
+  const float* scale;
+  const int* offsets;
+  const bf16* bias;
+  bf16* y;
+  int R, E, N, K, block;
+  int kw, nw, rows;       // warps per group, groups, most rows of a CTA
+};
+
+// STEP: 64 (the scale's block is a multiple of 64) or 32. WHOLE: the steps are whole pieces. DEPTH: pieces in a warp's ring.
+template <bool NF4, int STEP, bool WHOLE, int DEPTH>
+__global__ void __launch_bounds__(kMaxWarps * 32, 1) linear_4bit_kernel(const Args4 p) {
+  constexpr int kWords = STEP / 32;           // 32-bit words of codes per lane, weight row and step
+  constexpr int kRow = kU * STEP / 2;         // bytes of a piece's weight row: 128 or 64
+  constexpr int kChunks = kRow / 16, kCopies = 16 * kChunks / 32;
+  constexpr int kPiece = 16 * kRow + 16 * kU * 4;
+  extern __shared__ __align__(16) uint8_t sm4[];
+  const int r0 = p.offsets ? (int)blockIdx.y : (int)blockIdx.y * p.rows;
+  const Segment sg = segment_of(p.offsets, p.E, p.R, r0, p.rows);
+  if (sg.rows == 0) return;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
   if (sg.rows < 0) {
-    if (lane == 0) y[(long long)r0 * N + n] = __float2bfloat16(0.f);
+    for (int n = blockIdx.x * blockDim.x + threadIdx.x; n < p.N; n += gridDim.x * blockDim.x) p.y[(long long)r0 * p.N + n] = __float2bfloat16(0.f);
     return;
   }
-  const uint8_t* q = codes + ((long long)sg.e * N + n) * (K >> 1);
-  const float* sc = scale + ((long long)sg.e * N + n) * (K / block);
-  float acc[kRows];
+  const int M = sg.rows, steps = p.K / STEP, warps = p.kw * p.nw;
+  // The table and the zeros are static so that their addresses are constants of the loads.
+  __shared__ __align__(128) uint8_t table[NF4 ? kTable : 16];
+  __shared__ uint4 zero16;
+  uint8_t* ring = sm4 + warp * DEPTH * kPiece;
+  float* red = reinterpret_cast<float*>(sm4 + warps * DEPTH * kPiece);       // [2][warps][8][kRedRow]
+  uint8_t* xs = reinterpret_cast<uint8_t*>(red + 2 * warps * 8 * kRedRow);   // [step][kWords][M][4 lanes] 16 bytes
+  float* xscale = reinterpret_cast<float*>(xs + (size_t)steps * kWords * M * 64);      // [step][8] (NF4)
+
+  const int wg = warp / p.kw, wk = warp % p.kw;
+  const int pieces = (steps + kU - 1) / kU, p_lo = pieces * wk / p.kw, p_hi = pieces * (wk + 1) / p.kw;
+  const int spr = p.K / p.block, ratio = p.block / STEP;
+  const uint32_t k_bytes = (uint32_t)p.K >> 1;
+  const int tiles = (p.N + 15) / 16, stride = gridDim.x * p.nw;
+
+  // The ring: copy i of a lane is chunk lane % kChunks of weight row i * (32 / kChunks) + lane / kChunks; chunks are permuted by the row
+  // so that the eight rows that a read touches lie in different banks. Behind the codes the scales, [row][step]. Rows behind the
+  // weight's end keep what the ring holds: they are rows of their own in A and in the result, which is not stored.
+  const int c_row = lane / kChunks, c_chunk = lane % kChunks;
+  const uint32_t ring_u32 = smem_u32(ring);
+  const uint32_t c_dst = ring_u32 + c_row * kRow + ((c_chunk ^ (STEP == 64 ? (c_row << 1) & 7 : (c_row >> 1) & 3)) << 4);
+  const uint8_t* c_src = p.codes + ((long long)sg.e * p.N + c_row) * k_bytes + c_chunk * 16 + p_lo * kRow;
+  const float* s_src = p.scale + ((long long)sg.e * p.N + g) * spr;
+  const uint32_t c_step = (uint32_t)(32 / kChunks) * k_bytes, s_dst = ring_u32 + 16 * kRow + lane * 4;
+  int ft = blockIdx.x * p.nw + wg, fp = p_lo;          // next piece to fetch
+  const long long c_tile = 16ll * stride * k_bytes, s_tile = 16ll * stride * spr;     // from one tile of this warp to its next
+  c_src += 16ll * ft * k_bytes;
+  s_src += 16ll * ft * spr;
+  uint32_t fs = 0;                                     // its place in the ring, bytes
+  auto fetch = [&]() {
+    if (ft < tiles) {
+      const int s0 = fp * kU, si = ratio == 1 ? s0 + t : (s0 + t) / ratio;
+      const int left = p.N - ft * 16;                  // weight rows from here on
+      const uint8_t* src = c_src;
 #pragma unroll
-  for (int m = 0; m < kRows; ++m) acc[m] = 0.f;
-  for (int k = lane * 8; k < K; k += 256) {
-    const uint32_t c = *reinterpret_cast<const uint32_t*>(q + (k >> 1));
-    const float s = sc[k / block];
-    float w[8];
+      for (int i = 0; i < kCopies; ++i, src += c_step)
+        if ((WHOLE || (fp * kRow + c_chunk * 16) < (int)k_bytes) && (left >= 16 || i * (32 / kChunks) + c_row < left)) copy16(c_dst + fs + i * 512, src);
 #pragma unroll
-    for (int j = 0; j < 8; ++j) w[j] = lv[(c >> (4 * j)) & 15] * s;
-#pragma unroll
-    for (int m = 0; m < kRows; ++m)
-      if (m < sg.rows) {
-        float v[8];
-        unpack8(*reinterpret_cast<const bf16x8*>(x + (long long)(r0 + m) * ldx + k), v);
-#pragma unroll
-        for (int j = 0; j < 8; ++j) acc[m] = fmaf(w[j], v[j], acc[m]);
+      for (int h = 0; h < 2; ++h)
+        if ((WHOLE || s0 + t < steps) && (left >= 16 || g + 8 * h < left)) copy4(s_dst + fs + 128 * h, s_src + (h ? 8 * spr : 0) + si);
+      c_src += kRow;
+      if (++fp == p_hi) {
+        fp = p_lo;
+        ft += stride;
+        c_src += c_tile - (p_hi - p_lo) * kRow;
+        s_src += s_tile;
       }
-  }
+    }
+    fs = fs + kPiece == DEPTH * kPiece ? 0u : fs + kPiece;
+    copy_commit();                                     // also an empty group, so that groups count pieces
+  };
 #pragma unroll
-  for (int m = 0; m < kRows; ++m) {
-    const float s = warp_sum(acc[m]) + (bias ? __bfloat162float(bias[n]) : 0.f);
-    if (lane == 0 && m < sg.rows) y[(long long)(r0 + m) * N + n] = __float2bfloat16(s);
+  for (int i = 0; i < DEPTH - 1; ++i) fetch();
+
+  if (threadIdx.x == 0) zero16 = make_uint4(0, 0, 0, 0);
+  if (NF4) {
+    for (int i = threadIdx.x; i < 256 * 8; i += blockDim.x) {           // four lanes' copies of a pair at a time
+      const uint32_t v = half2_bits(c_level[1][(i >> 3) & 15], c_level[1][i >> 7]);
+      reinterpret_cast<uint4*>(table)[i] = make_uint4(v, v, v, v);
+    }
+  }
+  // x in the order of the codes: a quad of lanes per row and step
+  for (int i = threadIdx.x; i < steps * M * 4; i += blockDim.x) {
+    const int st = i / (4 * M), m = (i >> 2) % M, q = i & 3;      // a warp's 32 items keep whole quads
+    const bf16* src = p.x + (long long)(r0 + m) * p.ldx + st * STEP + q * (STEP / 4);
+    float v[kWords][8], f = 1.f;
+#pragma unroll
+    for (int w = 0; w < kWords; ++w) unpack8(*reinterpret_cast<const bf16x8*>(src + w * 8), v[w]);
+    const unsigned quad = 0xfu << (lane & ~3);
+    if (NF4) {
+      uint32_t top = 0;
+#pragma unroll
+      for (int w = 0; w < kWords; ++w)
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          const uint32_t b = __float_as_uint(v[w][j]) & 0x7fffffffu;
+          if (b < 0x7f800000u) top = max(top, b);
+        }
+      top = max(top, __shfl_xor_sync(quad, top, 1));
+      top = max(top, __shfl_xor_sync(quad, top, 2));
+      const int e = max((int)(top >> 23) - 127, -112);
+      f = __uint_as_float((uint32_t)(14 - e + 127) << 23);
+      if (q == 0) xscale[st * 8 + m] = __uint_as_float((uint32_t)(e - 14 + 127) << 23);
+    }
+#pragma unroll
+    for (int w = 0; w < kWords; ++w) {
+      uint4 o;
+      if (NF4)
+        o = make_uint4(half2_bits(v[w][0] * f, v[w][1] * f), half2_bits(v[w][2] * f, v[w][3] * f), half2_bits(v[w][4] * f, v[w][5] * f),
+                       half2_bits(v[w][6] * f, v[w][7] * f));
+      else
+        o = make_uint4(pack_bf162(v[w][0], v[w][4]), pack_bf162(v[w][1], v[w][5]), pack_bf162(v[w][2], v[w][6]), pack_bf162(v[w][3], v[w][7]));
+      *reinterpret_cast<uint4*>(xs + ((size_t)(st * kWords + w) * M * 4 + m * 4 + q) * 16) = o;
+    }
+  }
+  __syncthreads();
+
+  const uint32_t lane4 = lane * 4;
+  // this lane's x of a step; lanes of absent columns read zeros
+  const bool col = g < M;
+  const uint32_t x_step = col ? (uint32_t)(kWords * M * 64) : 0u, x_word = col ? (uint32_t)(M * 64) : 0u;
+  const uint8_t* x_lane = col ? xs + (size_t)p_lo * kU * kWords * M * 64 + g * 64 + t * 16 : reinterpret_cast<const uint8_t*>(&zero16);
+  // this lane's codes of step u in weight row g of a piece; row g + 8 is permuted alike
+  const uint8_t* q_row = ring + g * kRow;
+  uint32_t q_off[kU];
+#pragma unroll
+  for (int u = 0; u < kU; ++u)
+    q_off[u] = STEP == 64 ? (((2 * u + (t >> 1)) ^ ((g << 1) & 7)) << 4) + (t & 1) * 8 : ((u ^ ((g >> 1) & 3)) << 4) + t * 4;
+  const uint8_t* s_row = ring + 16 * kRow + g * 16;
+  uint32_t cs = 0;                                     // place in the ring of the piece being read
+  int buf = 0, turn = 0;                               // turn: warp that adds up this round, another one every time
+  // all warps of a CTA walk the same number of tiles, so that the barrier below is met by all
+  const int rounds = (tiles - (int)blockIdx.x * p.nw + stride - 1) / stride;
+  int tile = blockIdx.x * p.nw + wg;
+  for (int r = 0; r < rounds; ++r, tile += stride) {
+    float acc[4] = {0.f, 0.f, 0.f, 0.f};
+    if (tile < tiles) {
+      const uint8_t* xp = x_lane;
+      const float* xc_lane = xscale + p_lo * kU * 8 + 2 * t;
+#pragma unroll 1
+      for (int pc = p_lo; pc < p_hi; ++pc) {
+        copy_wait<DEPTH - 2>();
+        __syncwarp();                                  // every lane's copies of this piece have landed, the piece before has been read
+        fetch();
+        const float4 sa = *reinterpret_cast<const float4*>(s_row + cs), sb = *reinterpret_cast<const float4*>(s_row + cs + 128);
+        const float fa[4] = {sa.x, sa.y, sa.z, sa.w}, fb[4] = {sb.x, sb.y, sb.z, sb.w};
+#pragma unroll
+        for (int u = 0; u < kU; ++u) {
+          if (WHOLE || pc * kU + u < steps) {
+            float part[4] = {0.f, 0.f, 0.f, 0.f};
+            uint32_t c0[kWords], c1[kWords];
+            const uint8_t* q = q_row + cs + q_off[u];
+            if constexpr (kWords == 2) {
+              const uint2 a = *reinterpret_cast<const uint2*>(q), b = *reinterpret_cast<const uint2*>(q + 8 * kRow);
+              c0[0] = a.x; c0[kWords - 1] = a.y;
+              c1[0] = b.x; c1[kWords - 1] = b.y;
+            } else {
+              c0[0] = *reinterpret_cast<const uint32_t*>(q);
+              c1[0] = *reinterpret_cast<const uint32_t*>(q + 8 * kRow);
+            }
+#pragma unroll
+            for (int w = 0; w < kWords; ++w) {
+              const uint4 b = *reinterpret_cast<const uint4*>(xp + w * x_word);
+              uint32_t h0[4], h1[4];
+              decode8<NF4>(c0[w], table, lane4, h0);
+              decode8<NF4>(c1[w], table, lane4, h1);
+              mma16816<NF4>(part, h0[0], h1[0], h0[1], h1[1], b.x, b.y);
+              mma16816<NF4>(part, h0[2], h1[2], h0[3], h1[3], b.z, b.w);
+            }
+            xp += x_step;
+            if (NF4) {
+              const float2 xc = *reinterpret_cast<const float2*>(xc_lane + u * 8);
+              part[0] *= xc.x; part[1] *= xc.y; part[2] *= xc.x; part[3] *= xc.y;
+            }
+            acc[0] = fmaf(part[0], fa[u], acc[0]);
+            acc[1] = fmaf(part[1], fa[u], acc[1]);
+            acc[2] = fmaf(part[2], fb[u], acc[2]);
+            acc[3] = fmaf(part[3], fb[u], acc[3]);
+          }
+        }
+        xc_lane += kU * 8;
+        cs = cs + kPiece == DEPTH * kPiece ? 0u : cs + kPiece;
+      }
+    }
+    float* mine = red + (buf * warps + warp) * 8 * kRedRow + 2 * t * kRedRow + g;
+    mine[0] = acc[0];
+    mine[kRedRow] = acc[1];
+    mine[8] = acc[2];
+    mine[kRedRow + 8] = acc[3];
+    __syncthreads();
+    int i = threadIdx.x - turn * 32;
+    turn = turn + 1 == warps ? 0 : turn + 1;
+    for (i += i < 0 ? warps * 32 : 0; i < p.nw * M * 16; i += warps * 32) {
+      const int row = i & 15, m = p.nw == 1 ? i >> 4 : (i >> 4) % M, grp = p.nw == 1 ? 0 : (i >> 4) / M;
+      const int n = ((blockIdx.x + r * gridDim.x) * p.nw + grp) * 16 + row;
+      if (n < p.N) {
+        const float* src = red + ((buf * p.nw + grp) * p.kw * 8 + m) * kRedRow + row;
+        float v = 0.f;
+#pragma unroll 4
+        for (int q = 0; q < p.kw; ++q) v += src[q * 8 * kRedRow];
+        if (!NF4) v *= 1.f / 7.f;
+        if (p.bias) v += __bfloat162float(p.bias[n]);
+        p.y[(long long)(r0 + m) * p.N + n] = __float2bfloat16(v);
+      }
+    }
+    buf ^= 1;       // the next round writes the other half; the barrier there is behind these reads
   }
 }
 
@@ -86,7 +324,7 @@ __global__ void __launch_bounds__(128) dgrad_4bit_kernel(const bf16* __restrict_
                                                          const float* __restrict__ scale, const int* __restrict__ offsets,
                                                          float* __restrict__ part, int R, int E, int N, int K, int block, int nf4) {
   const int r0 = blockIdx.y;
-  const Segment sg = segment_of(offsets, E, R, r0);
+  const Segment sg = segment_of(offsets, E, R, r0, kRows);
   if (sg.rows == 0) return;
   __shared__ float lv[16];
   if (threadIdx.x < 16) lv[threadIdx.x] = c_level[nf4][threadIdx.x];
@@ -146,6 +384,43 @@ bool dims_ok(int R, int E, int N, int K, int block) {
   return R >= 1 && R <= 65535 && E >= 1 && N >= 1 && block >= 32 && block % 32 == 0 && K >= block && K % block == 0;
 }
 
+constexpr int kSmem4 = 227 * 1024 - 1024;       // of an SM, one CTA
+int min_of(int a, int b) { return a < b ? a : b; }
+
+template <bool NF4, int STEP, bool WHOLE, int DEPTH>
+int launch4d(const Args4& p, dim3 grid, int smem, int dev, cudaStream_t st) {
+  static bool configured[64] = {};
+  if (!configured[dev]) {
+    const cudaError_t e = cudaFuncSetAttribute(linear_4bit_kernel<NF4, STEP, WHOLE, DEPTH>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                               kSmem4 - (NF4 ? kTable : 0));
+    if (e != cudaSuccess) return (int)e;
+    configured[dev] = true;
+  }
+  linear_4bit_kernel<NF4, STEP, WHOLE, DEPTH><<<grid, p.kw * p.nw * 32, smem, st>>>(p);
+  return (int)cudaGetLastError();
+}
+
+template <bool NF4, int STEP>
+int launch4(Args4& p, int dev, cudaStream_t st) {
+  const int steps = p.K / STEP, pieces = (steps + kU - 1) / kU, turns = (pieces + kMaxWarps - 1) / kMaxWarps, tiles = (p.N + 15) / 16;
+  p.kw = (pieces + turns - 1) / turns;
+  p.nw = min_of(kMaxWarps / p.kw, tiles);
+  // shared memory: the table, every warp's ring, partial sums, x of the CTA's rows. A ring of three pieces where all rows of x fit
+  // next to it, else two; fewer rows per CTA (the codes are then read again, from L2) where a long x fits neither way.
+  const int warps = p.kw * p.nw, piece = 16 * kU * STEP / 2 + 16 * kU * 4, fixed = 2 * warps * 8 * kRedRow * 4 + (NF4 ? steps * 32 : 0);
+  const int room = kSmem4 - (NF4 ? kTable : 0) - fixed, want = min_of(kRows, p.R);
+  const int depth = room - 3 * warps * piece >= want * 2 * p.K ? 3 : 2;
+  p.rows = min_of(want, (room - depth * warps * piece) / (2 * p.K));
+  if (p.rows < 1) return -100;
+  const int smem = fixed + depth * warps * piece + p.rows * 2 * p.K;
+  // one CTA per SM; of the rows that may start a CTA in the grouped form (known on the device only) half are taken to
+  const int most = (tiles + p.nw - 1) / p.nw, share = p.offsets ? (148 * 2 + p.R - 1) / p.R : 148;
+  const dim3 grid(min_of(most, share), p.offsets ? p.R : (p.R + p.rows - 1) / p.rows);
+  const bool whole = steps % kU == 0;
+  if (depth == 3) return whole ? launch4d<NF4, STEP, true, 3>(p, grid, smem, dev, st) : launch4d<NF4, STEP, false, 3>(p, grid, smem, dev, st);
+  return whole ? launch4d<NF4, STEP, true, 2>(p, grid, smem, dev, st) : launch4d<NF4, STEP, false, 2>(p, grid, smem, dev, st);
+}
+
 }  // namespace
 
 extern "C" {
@@ -154,9 +429,12 @@ extern "C" {
 int eri_linear_4bit(const void* x, long long ldx, const void* codes, const float* scale, const int* offsets, const void* bias, void* y, int R, int E,
                     int N, int K, int block, int nf4, void* stream) {
   if (!dims_ok(R, E, N, K, block) || (bias && offsets) || ldx % 8 || (((uintptr_t)x | (uintptr_t)codes) & 15)) return -1;
-  linear_4bit_kernel<<<dim3((N + 7) / 8, R), 256, 0, (cudaStream_t)stream>>>((const bf16*)x, ldx, (const uint8_t*)codes, scale, offsets,
-                                                                             (const bf16*)bias, (bf16*)y, R, E, N, K, block, nf4 ? 1 : 0);
-  return (int)cudaGetLastError();
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return -2;
+  Args4 p = {(const bf16*)x, ldx, (const uint8_t*)codes, scale, offsets, (const bf16*)bias, (bf16*)y, R, E, N, K, block, 0, 0, 0};
+  cudaStream_t st = (cudaStream_t)stream;
+  if (block % 64 == 0) return nf4 ? launch4<true, 64>(p, dev, st) : launch4<false, 64>(p, dev, st);
+  return nf4 ? launch4<true, 32>(p, dev, st) : launch4<false, 32>(p, dev, st);
 }
 
 // Planes of the workspace [planes, R, K] fp32 that eri_linear_4bit_dgrad wants.
