@@ -114,13 +114,72 @@ struct Args4 {
   int kw, nw, rows;       // warps per group, groups, most rows of a CTA
 };
 
-// STEP: 64 (the scale's block is a multiple of 64) or 32. WHOLE: the steps are whole pieces. DEPTH: pieces in a warp's ring.
+// A warp's ring of pieces: kU steps (128 or 64 bytes) of 16 weight rows, 16-byte chunks permuted by the row so that reads of eight rows
+// two apart or of four rows one apart hit different banks, and behind them the scales, [row][step]. Pieces are copied
+// asynchronously, DEPTH - 1 ahead of the one being read; one commit group per piece.
+// STEP: 64 (the scale's block is a multiple of 64) or 32. WHOLE: K is whole pieces.
+template <int STEP, bool WHOLE, int DEPTH>
+struct PieceRing {
+  static constexpr int kRow = kU * STEP / 2;                  // bytes of a weight row in a piece
+  static constexpr int kChunks = kRow / 16, kCopies = 16 * kChunks / 32;
+  static constexpr int kPiece = 16 * kRow + 16 * kU * 4;
+  static constexpr int kBytes = DEPTH * kPiece;
+  const uint8_t* src;         // this lane's chunk of the next piece
+  const float* s_src;
+  long long tile_bytes, tile_scales;
+  uint32_t dst, s_dst, row_step, at;
+  int tile, piece, tile_end, tile_step, p_lo, p_hi;
+  int N, k_bytes, spr, ratio, steps, lane;
+
+  // pieces p_lo .. p_hi - 1 of the 16-row tiles first, first + step, ... below end
+  __device__ __forceinline__ PieceRing(const uint8_t* codes, const float* scale, int N_, int K, int block, uint32_t smem, int lane_,
+                                       int first, int end, int step, int lo, int hi)
+      : at(0), tile(first), piece(lo), tile_end(end), tile_step(step), p_lo(lo), p_hi(hi), N(N_), k_bytes(K >> 1), spr(K / block),
+        ratio(block / STEP), steps(K / STEP), lane(lane_) {
+    const int row = lane / kChunks, chunk = lane % kChunks;
+    dst = smem + row * kRow + (place(row, chunk) << 4);
+    s_dst = smem + 16 * kRow + lane * 4;
+    row_step = (uint32_t)(32 / kChunks) * k_bytes;
+    tile_bytes = 16ll * step * k_bytes - (long long)(hi - lo) * kRow;
+    tile_scales = 16ll * step * spr;
+    src = codes + (16ll * first + row) * k_bytes + lo * kRow + chunk * 16;
+    s_src = scale + (16ll * first + (lane >> 2)) * spr;
+  }
+  // chunk's place in its row
+  static __device__ __forceinline__ int place(int row, int chunk) {
+    return STEP == 64 ? chunk ^ ((row << 1) & 7) : chunk ^ ((row >> 1) & 3);
+  }
+  __device__ __forceinline__ void fetch() {
+    if (tile < tile_end) {
+      const int row = lane / kChunks, chunk = lane % kChunks, g = lane >> 2, t = lane & 3;
+      const int s0 = piece * kU, si = ratio == 1 ? s0 + t : (s0 + t) / ratio;
+      const int left = N - tile * 16;                          // weight rows from here on
+      const uint8_t* q = src;
+#pragma unroll
+      for (int i = 0; i < kCopies; ++i, q += row_step)
+        if ((WHOLE || piece * kRow + chunk * 16 < k_bytes) && (left >= 16 || i * (32 / kChunks) + row < left)) copy16(dst + at + i * 512, q);
+#pragma unroll
+      for (int h = 0; h < 2; ++h)                             // behind the last row its scales again: they have to be numbers
+        if (WHOLE || s0 + t < steps)
+          copy4(s_dst + at + 128 * h, s_src + (left >= 16 || g + 8 * h < left ? 8 * h : left - 1 - g) * spr + si);
+      src += kRow;
+      if (++piece == p_hi) {
+        piece = p_lo;
+        tile += tile_step;
+        src += tile_bytes;
+        s_src += tile_scales;
+      }
+    }
+    at = at + kPiece == kBytes ? 0u : at + kPiece;
+    copy_commit();                                            // also an empty group, so that groups count pieces
+  }
+};
+
 template <bool NF4, int STEP, bool WHOLE, int DEPTH>
 __global__ void __launch_bounds__(kMaxWarps * 32, 1) linear_4bit_kernel(const Args4 p) {
+  using Ring = PieceRing<STEP, WHOLE, DEPTH>;
   constexpr int kWords = STEP / 32;           // 32-bit words of codes per lane, weight row and step
-  constexpr int kRow = kU * STEP / 2;         // bytes of a piece's weight row: 128 or 64
-  constexpr int kChunks = kRow / 16, kCopies = 16 * kChunks / 32;
-  constexpr int kPiece = 16 * kRow + 16 * kU * 4;
+  constexpr int kRow = Ring::kRow, kPiece = Ring::kPiece;
   extern __shared__ __align__(16) uint8_t sm4[];
   const int r0 = p.offsets ? (int)blockIdx.y : (int)blockIdx.y * p.rows;
   const Segment sg = segment_of(p.offsets, p.E, p.R, r0, p.rows);
@@ -141,48 +200,11 @@ __global__ void __launch_bounds__(kMaxWarps * 32, 1) linear_4bit_kernel(const Ar
 
   const int wg = warp / p.kw, wk = warp % p.kw;
   const int pieces = (steps + kU - 1) / kU, p_lo = pieces * wk / p.kw, p_hi = pieces * (wk + 1) / p.kw;
-  const int spr = p.K / p.block, ratio = p.block / STEP;
-  const uint32_t k_bytes = (uint32_t)p.K >> 1;
   const int tiles = (p.N + 15) / 16, stride = gridDim.x * p.nw;
-
-  // The ring: copy i of a lane is chunk lane % kChunks of weight row i * (32 / kChunks) + lane / kChunks; chunks are permuted by the row
-  // so that the eight rows that a read touches lie in different banks. Behind the codes the scales, [row][step]. Rows behind the
-  // weight's end keep what the ring holds: they are rows of their own in A and in the result, which is not stored.
-  const int c_row = lane / kChunks, c_chunk = lane % kChunks;
-  const uint32_t ring_u32 = smem_u32(ring);
-  const uint32_t c_dst = ring_u32 + c_row * kRow + ((c_chunk ^ (STEP == 64 ? (c_row << 1) & 7 : (c_row >> 1) & 3)) << 4);
-  const uint8_t* c_src = p.codes + ((long long)sg.e * p.N + c_row) * k_bytes + c_chunk * 16 + p_lo * kRow;
-  const float* s_src = p.scale + ((long long)sg.e * p.N + g) * spr;
-  const uint32_t c_step = (uint32_t)(32 / kChunks) * k_bytes, s_dst = ring_u32 + 16 * kRow + lane * 4;
-  int ft = blockIdx.x * p.nw + wg, fp = p_lo;          // next piece to fetch
-  const long long c_tile = 16ll * stride * k_bytes, s_tile = 16ll * stride * spr;     // from one tile of this warp to its next
-  c_src += 16ll * ft * k_bytes;
-  s_src += 16ll * ft * spr;
-  uint32_t fs = 0;                                     // its place in the ring, bytes
-  auto fetch = [&]() {
-    if (ft < tiles) {
-      const int s0 = fp * kU, si = ratio == 1 ? s0 + t : (s0 + t) / ratio;
-      const int left = p.N - ft * 16;                  // weight rows from here on
-      const uint8_t* src = c_src;
+  Ring feed(p.codes + (long long)sg.e * p.N * (p.K >> 1), p.scale + (long long)sg.e * p.N * (p.K / p.block), p.N, p.K, p.block, smem_u32(ring),
+            lane, blockIdx.x * p.nw + wg, tiles, stride, p_lo, p_hi);
 #pragma unroll
-      for (int i = 0; i < kCopies; ++i, src += c_step)
-        if ((WHOLE || (fp * kRow + c_chunk * 16) < (int)k_bytes) && (left >= 16 || i * (32 / kChunks) + c_row < left)) copy16(c_dst + fs + i * 512, src);
-#pragma unroll
-      for (int h = 0; h < 2; ++h)
-        if ((WHOLE || s0 + t < steps) && (left >= 16 || g + 8 * h < left)) copy4(s_dst + fs + 128 * h, s_src + (h ? 8 * spr : 0) + si);
-      c_src += kRow;
-      if (++fp == p_hi) {
-        fp = p_lo;
-        ft += stride;
-        c_src += c_tile - (p_hi - p_lo) * kRow;
-        s_src += s_tile;
-      }
-    }
-    fs = fs + kPiece == DEPTH * kPiece ? 0u : fs + kPiece;
-    copy_commit();                                     // also an empty group, so that groups count pieces
-  };
-#pragma unroll
-  for (int i = 0; i < DEPTH - 1; ++i) fetch();
+  for (int i = 0; i < DEPTH - 1; ++i) feed.fetch();
 
   if (threadIdx.x == 0) zero16 = make_uint4(0, 0, 0, 0);
   if (NF4) {
@@ -253,7 +275,7 @@ __global__ void __launch_bounds__(kMaxWarps * 32, 1) linear_4bit_kernel(const Ar
       for (int pc = p_lo; pc < p_hi; ++pc) {
         copy_wait<DEPTH - 2>();
         __syncwarp();                                  // every lane's copies of this piece have landed, the piece before has been read
-        fetch();
+        feed.fetch();
         const float4 sa = *reinterpret_cast<const float4*>(s_row + cs), sb = *reinterpret_cast<const float4*>(s_row + cs + 128);
         const float fa[4] = {sa.x, sa.y, sa.z, sa.w}, fb[4] = {sb.x, sb.y, sb.z, sb.w};
 #pragma unroll
@@ -319,49 +341,183 @@ __global__ void __launch_bounds__(kMaxWarps * 32, 1) linear_4bit_kernel(const Ar
   }
 }
 
-// A thread owns eight columns and walks the weight rows of its split; the splits' planes are added in order by the second kernel.
-__global__ void __launch_bounds__(128) dgrad_4bit_kernel(const bf16* __restrict__ dy, long long ldy, const uint8_t* __restrict__ codes,
-                                                         const float* __restrict__ scale, const int* __restrict__ offsets,
-                                                         float* __restrict__ part, int R, int E, int N, int K, int block, int nf4) {
-  const int r0 = blockIdx.y;
-  const Segment sg = segment_of(offsets, E, R, r0, kRows);
-  if (sg.rows == 0) return;
-  __shared__ float lv[16];
-  if (threadIdx.x < 16) lv[threadIdx.x] = c_level[nf4][threadIdx.x];
-  __syncthreads();
-  const int k = (blockIdx.x * 128 + threadIdx.x) * 8;
-  if (k >= K) return;
-  const int rows = sg.rows < 0 ? 1 : sg.rows;
-  float acc[kRows][8];
+// ------------------------------------------------------------------------------------------- dx = dy W
+// The reduction runs over the weight rows n, and every block of a row has a scale of its own: dy[m, n] scale[n, block] is formed in 32 bits
+// for each block and becomes the B operand (16 weight rows x 8 rows of dy) of the block's products; A are the levels of 16 columns of
+// W, one register holding two weight rows of one column. Both are fp16: int4 codes - 8 are exact, NF4 levels and dy * scale
+// are rounded to 2^-12 of themselves. A power of two per row of dy keeps dy * scale in fp16's range: the first 16 weight rows
+// place its largest magnitude at 2^8, and when a later one would pass 2^15 the sums are scaled down with it (rare). Values down to
+// 2^-22 of the largest keep all their bits, the rest is off by 2^-33 of it.
+// A CTA owns one piece of columns (256, or 128 with blocks of 32) and a range of weight rows; its warps take every kDgWarps-th 16 rows, their
+// sums meet in shared memory in warp order, and the ranges' planes are added in order by the kernel below.
+constexpr int kDgWarps = 16, kDgDepth = 3, kDgRows = 2048;        // kDgRows: most weight rows of a range (their dy is in shared memory)
+
+template <bool NF4>
+__device__ __forceinline__ void decode_rows(uint32_t a, uint32_t b, const uint8_t (&table)[NF4 ? kTable : 16], uint32_t lane4, uint32_t (&h)[8]) {
+  // h[i]: code i of word a in the low half, of word b in the high half
+  if constexpr (NF4) {
+    const uint32_t even = (a & 0x0f0f0f0fu) | ((b << 4) & 0xf0f0f0f0u), odd = ((a >> 4) & 0x0f0f0f0fu) | (b & 0xf0f0f0f0u);
 #pragma unroll
-  for (int m = 0; m < kRows; ++m)
+    for (int i = 0; i < 4; ++i) {
+      h[2 * i] = *reinterpret_cast<const uint32_t*>(table + (((i == 0 ? even << 7 : even >> (8 * i - 7)) & 0x7f80u) | lane4));
+      h[2 * i + 1] = *reinterpret_cast<const uint32_t*>(table + (((i == 0 ? odd << 7 : odd >> (8 * i - 7)) & 0x7f80u) | lane4));
+    }
+  } else {
+    const uint32_t lo = __byte_perm(a, b, 0x5410), hi = __byte_perm(a, b, 0x7632);
+    const __half2 off = __floats2half2_rn(1032.f, 1032.f);                // 1024 + code - 1032, exact
 #pragma unroll
-    for (int j = 0; j < 8; ++j) acc[m][j] = 0.f;
-  if (sg.rows > 0) {
-    const int n0 = (int)((long long)N * blockIdx.z / gridDim.z), n1 = (int)((long long)N * (blockIdx.z + 1) / gridDim.z);
-    for (int n = n0; n < n1; ++n) {
-      const long long row = (long long)sg.e * N + n;
-      const uint32_t c = *reinterpret_cast<const uint32_t*>(codes + row * (K >> 1) + (k >> 1));
-      const float s = scale[row * (K / block) + k / block];
-      float w[8];
-#pragma unroll
-      for (int j = 0; j < 8; ++j) w[j] = lv[(c >> (4 * j)) & 15] * s;
-#pragma unroll
-      for (int m = 0; m < kRows; ++m)
-        if (m < rows) {
-          const float d = __bfloat162float(dy[(long long)(r0 + m) * ldy + n]);
-#pragma unroll
-          for (int j = 0; j < 8; ++j) acc[m][j] = fmaf(d, w[j], acc[m][j]);
-        }
+    for (int i = 0; i < 8; ++i) {
+      uint32_t v = (((i < 4 ? lo : hi) >> (4 * (i & 3))) & 0x000f000fu) | 0x64006400u;
+      const __half2 w = __hsub2(*reinterpret_cast<__half2*>(&v), off);
+      h[i] = *reinterpret_cast<const uint32_t*>(&w);
     }
   }
+}
+
+struct DgArgs {
+  const bf16* dy;
+  long long ldy;
+  const uint8_t* codes;
+  const float* scale;
+  const int* offsets;
+  float* part;
+  int R, E, N, K, block;
+};
+
+template <bool NF4, int STEP, bool WHOLE>
+__global__ void __launch_bounds__(kDgWarps * 32, 1) dgrad_4bit_kernel(const DgArgs p) {
+  using Ring = PieceRing<STEP, WHOLE, kDgDepth>;
+  constexpr int kHalves = STEP / 32;                    // groups of four codes per lane, weight row and step
+  constexpr int kCols = kU * STEP;                      // columns of the CTA
+  constexpr int kRow = Ring::kRow, kPiece = Ring::kPiece;
+  extern __shared__ __align__(16) uint8_t sm4[];
+  __shared__ __align__(128) uint8_t table[NF4 ? kTable : 16];
+  const int r0 = p.offsets ? (int)blockIdx.y : (int)blockIdx.y * kRows;
+  const Segment sg = segment_of(p.offsets, p.E, p.R, r0, kRows);
+  if (sg.rows == 0) return;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+  const int k0 = blockIdx.x * kCols;
+  const int M = sg.rows < 0 ? 1 : sg.rows, steps = p.K / STEP;
+  float* plane = p.part + ((long long)blockIdx.z * p.R + r0) * p.K;
+  if (sg.rows < 0) {
+    for (int k = k0 + threadIdx.x; k < min(k0 + kCols, p.K); k += blockDim.x) plane[k] = 0.f;
+    return;
+  }
+  const int tiles = (p.N + 15) / 16;
+  const int t_lo = (int)((long long)tiles * blockIdx.z / gridDim.z), t_hi = (int)((long long)tiles * (blockIdx.z + 1) / gridDim.z);
+  float* dys = reinterpret_cast<float*>(sm4);           // [weight rows of the range][8]
+  uint8_t* rings = sm4 + kDgRows * 32;
+  uint8_t* ring = rings + warp * Ring::kBytes;
+  Ring feed(p.codes + (long long)sg.e * p.N * (p.K >> 1), p.scale + (long long)sg.e * p.N * (p.K / p.block), p.N, p.K, p.block, smem_u32(ring),
+            lane, t_lo + warp, t_hi, kDgWarps, blockIdx.x, blockIdx.x + 1);
 #pragma unroll
-  for (int m = 0; m < kRows; ++m)
-    if (m < rows) {
-      float4* o = reinterpret_cast<float4*>(part + ((long long)blockIdx.z * R + r0 + m) * K + k);
-      o[0] = make_float4(acc[m][0], acc[m][1], acc[m][2], acc[m][3]);
-      o[1] = make_float4(acc[m][4], acc[m][5], acc[m][6], acc[m][7]);
+  for (int i = 0; i < kDgDepth - 1; ++i) feed.fetch();
+  if (NF4)
+    for (int i = threadIdx.x; i < 256 * 8; i += blockDim.x) {           // four lanes' copies of a pair at a time
+      const uint32_t v = half2_bits(c_level[1][(i >> 3) & 15], c_level[1][i >> 7]);
+      reinterpret_cast<uint4*>(table)[i] = make_uint4(v, v, v, v);
     }
+  for (int i = threadIdx.x; i < (t_hi - t_lo) * 16 * 8; i += blockDim.x) {
+    const int m = i / ((t_hi - t_lo) * 16), r = i - m * (t_hi - t_lo) * 16, n = t_lo * 16 + r;
+    dys[r * 8 + m] = m < M && n < p.N ? __bfloat162float(p.dy[(long long)(r0 + m) * p.ldy + n]) : 0.f;
+  }
+  __syncthreads();
+
+  const uint32_t lane4 = lane * 4;
+  float acc[kU][2 * kHalves][4];
+#pragma unroll
+  for (int u = 0; u < kU; ++u)
+#pragma unroll
+    for (int j = 0; j < 2 * kHalves; ++j) acc[u][j][0] = acc[u][j][1] = acc[u][j][2] = acc[u][j][3] = 0.f;
+  int top = -1000;                                      // exponent that stands at 2^8 in row g of dy
+  uint32_t cs = 0;
+  const int s_cta = blockIdx.x * kU;                    // first step of the CTA's columns
+#pragma unroll 1
+  for (int tile = t_lo + warp; tile < t_hi; tile += kDgWarps) {
+    copy_wait<kDgDepth - 2>();
+    __syncwarp();                                       // every lane's copies of this piece have landed, the piece before has been read
+    feed.fetch();
+    // this lane's weight rows of the tile are t, t + 4, t + 8, t + 12
+    float v[kU][4];
+    uint32_t big = 0;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const float d = dys[((tile - t_lo) * 16 + t + 4 * i) * 8 + g];
+      const float4 sc = *reinterpret_cast<const float4*>(ring + cs + 16 * kRow + (t + 4 * i) * 16);
+      v[0][i] = d * sc.x; v[1][i] = d * sc.y; v[2][i] = d * sc.z; v[3][i] = d * sc.w;
+#pragma unroll
+      for (int u = 0; u < kU; ++u) {
+        if (!WHOLE && s_cta + u >= steps) v[u][i] = 0.f;
+        const uint32_t b = __float_as_uint(v[u][i]) & 0x7fffffffu;
+        if (b < 0x7f800000u) big = max(big, b);
+      }
+    }
+    big = max(big, __shfl_xor_sync(0xffffffffu, big, 1));
+    big = max(big, __shfl_xor_sync(0xffffffffu, big, 2));
+    const int e = (int)(big >> 23) - 127;
+    const bool grow = big != 0 && e > top + 6;
+    if (__any_sync(0xffffffffu, grow)) {
+      // sums of the rows that grow are scaled down with them; the accumulator's columns are rows 2 t and 2 t + 1 of dy
+      const int to = grow ? max(e, -110) : top;
+      const int down = top - to;                        // <= 0; from "nothing yet" the sums are zeros (or not finite)
+      const float f = top < -110 ? 1.f : __uint_as_float((uint32_t)(127 + max(down, -126)) << 23);
+      top = to;
+      const float f0 = __shfl_sync(0xffffffffu, f, 8 * t), f1 = __shfl_sync(0xffffffffu, f, 8 * t + 4);
+#pragma unroll
+      for (int u = 0; u < kU; ++u)
+#pragma unroll
+        for (int j = 0; j < 2 * kHalves; ++j) {
+          acc[u][j][0] *= f0; acc[u][j][1] *= f1; acc[u][j][2] *= f0; acc[u][j][3] *= f1;
+        }
+    }
+    const float f = top < -110 ? 1.f : __uint_as_float((uint32_t)(127 + 8 - top) << 23);       // (nothing but zeros so far: any)
+#pragma unroll
+    for (int u = 0; u < kU; ++u) {
+      if (WHOLE || s_cta + u < steps) {
+        const uint32_t b0 = half2_bits(v[u][0] * f, v[u][1] * f), b1 = half2_bits(v[u][2] * f, v[u][3] * f);
+        uint32_t w[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const int row = t + 4 * i;
+          if constexpr (STEP == 64)
+            w[i] = *reinterpret_cast<const uint32_t*>(ring + cs + row * kRow + (Ring::place(row, 2 * u + (g >> 2)) << 4) + (g & 3) * 4);
+          else
+            w[i] = *reinterpret_cast<const uint16_t*>(ring + cs + row * kRow + (Ring::place(row, u) << 4) + g * 2);
+        }
+        uint32_t h0[8], h1[8];
+        decode_rows<NF4>(w[0], w[1], table, lane4, h0);
+        decode_rows<NF4>(w[2], w[3], table, lane4, h1);
+#pragma unroll
+        for (int j = 0; j < 2 * kHalves; ++j) mma16816<true>(acc[u][j], h0[2 * j], h0[2 * j + 1], h1[2 * j], h1[2 * j + 1], b0, b1);
+      }
+    }
+    cs = cs + kPiece == Ring::kBytes ? 0u : cs + kPiece;
+  }
+  // the rings and dy are read, and nothing is on its way into them: the memory takes the sums
+  copy_wait<0>();
+  __syncthreads();
+  constexpr int kPitch = kCols + 4;
+  float* red = reinterpret_cast<float*>(sm4) + warp * 8 * kPitch;         // [warp][8][kPitch]
+  const float back = top < -110 ? 0.f : __uint_as_float((uint32_t)(127 - 8 + max(top, -110)) << 23);
+  const float k0s = __shfl_sync(0xffffffffu, back, 8 * t) * (NF4 ? 1.f : 1.f / 7.f), k1s = __shfl_sync(0xffffffffu, back, 8 * t + 4) * (NF4 ? 1.f : 1.f / 7.f);
+#pragma unroll
+  for (int u = 0; u < kU; ++u)
+#pragma unroll
+    for (int j = 0; j < 2 * kHalves; ++j) {
+      const int k = u * STEP + g * (STEP / 8) + 2 * j;
+      *reinterpret_cast<float2*>(red + (2 * t) * kPitch + k) = make_float2(acc[u][j][0] * k0s, acc[u][j][2] * k0s);
+      *reinterpret_cast<float2*>(red + (2 * t + 1) * kPitch + k) = make_float2(acc[u][j][1] * k1s, acc[u][j][3] * k1s);
+    }
+  __syncthreads();
+  for (int i = threadIdx.x; i < M * kCols; i += blockDim.x) {
+    const int m = i / kCols, k = i % kCols;
+    if (k0 + k >= p.K) continue;
+    const float* q = reinterpret_cast<const float*>(sm4) + m * kPitch + k;
+    float s = 0.f;
+#pragma unroll
+    for (int w = 0; w < kDgWarps; ++w) s += q[w * 8 * kPitch];
+    plane[(long long)m * p.K + k0 + k] = s;
+  }
 }
 
 __global__ void __launch_bounds__(256) add_planes_kernel(const float* __restrict__ part, bf16* __restrict__ out, long long vecs,
@@ -421,6 +577,27 @@ int launch4(Args4& p, int dev, cudaStream_t st) {
   return whole ? launch4d<NF4, STEP, true, 2>(p, grid, smem, dev, st) : launch4d<NF4, STEP, false, 2>(p, grid, smem, dev, st);
 }
 
+template <bool NF4, int STEP, bool WHOLE>
+int launch_dgw(const DgArgs& p, int planes, int dev, cudaStream_t st) {
+  using Ring = PieceRing<STEP, WHOLE, kDgDepth>;
+  constexpr int kCols = kU * STEP, kRings = kDgWarps * Ring::kBytes, kRed = kDgWarps * 8 * (kCols + 4) * 4;
+  constexpr int kSmem = kDgRows * 32 + kRings > kRed ? kDgRows * 32 + kRings : kRed;
+  static_assert(kSmem + (NF4 ? kTable : 0) <= kSmem4, "shared memory of a CTA");
+  static bool configured[64] = {};
+  if (!configured[dev]) {
+    const cudaError_t e = cudaFuncSetAttribute(dgrad_4bit_kernel<NF4, STEP, WHOLE>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem);
+    if (e != cudaSuccess) return (int)e;
+    configured[dev] = true;
+  }
+  const dim3 grid((p.K + kCols - 1) / kCols, p.offsets ? p.R : (p.R + kRows - 1) / kRows, planes);
+  dgrad_4bit_kernel<NF4, STEP, WHOLE><<<grid, kDgWarps * 32, kSmem, st>>>(p);
+  return (int)cudaGetLastError();
+}
+template <bool NF4, int STEP>
+int launch_dg(const DgArgs& p, int planes, int dev, cudaStream_t st) {
+  return p.K % (kU * STEP) == 0 ? launch_dgw<NF4, STEP, true>(p, planes, dev, st) : launch_dgw<NF4, STEP, false>(p, planes, dev, st);
+}
+
 }  // namespace
 
 extern "C" {
@@ -437,23 +614,32 @@ int eri_linear_4bit(const void* x, long long ldx, const void* codes, const float
   return nf4 ? launch4<true, 32>(p, dev, st) : launch4<false, 32>(p, dev, st);
 }
 
-// Planes of the workspace [planes, R, K] fp32 that eri_linear_4bit_dgrad wants.
-int eri_linear_4bit_planes(int R, int N, int K) {
-  const int blocks = ((K / 8 + 127) / 128) * ((R + kRows - 1) / kRows);
-  int s = (148 * 8 + blocks - 1) / blocks;
-  if (s > (N + 31) / 32) s = (N + 31) / 32;
-  return s < 1 ? 1 : s > 64 ? 64 : s;
+// Planes of the workspace [planes, R, K] fp32 that eri_linear_4bit_dgrad wants: ranges of weight rows, so that the CTAs fill the SMs and a
+// range's dy fits shared memory.
+int eri_linear_4bit_planes(int R, int N, int K, int block, int grouped) {
+  const int cols = kU * (block % 64 == 0 ? 64 : 32), blocks = ((K + cols - 1) / cols) * (grouped ? (R + 1) / 2 : (R + kRows - 1) / kRows);
+  int s = 148 / blocks;
+  const int most = (N + 16 * kDgWarps - 1) / (16 * kDgWarps), least = ((N + 15) / 16 + kDgRows / 16 - 1) / (kDgRows / 16);
+  if (s > most) s = most;
+  if (s < least) s = least;
+  return s < 1 ? 1 : s;
 }
 
 // dy [R, N] (row stride ldy) -> dx [R, K] contiguous.
 int eri_linear_4bit_dgrad(const void* dy, long long ldy, const void* codes, const float* scale, const int* offsets, float* work, void* dx,
                           int R, int E, int N, int K, int block, int nf4, void* stream) {
   if (!dims_ok(R, E, N, K, block) || (((uintptr_t)dx | (uintptr_t)codes | (uintptr_t)work) & 15)) return -1;
-  const int planes = eri_linear_4bit_planes(R, N, K);
-  dgrad_4bit_kernel<<<dim3((K / 8 + 127) / 128, R, planes), 128, 0, (cudaStream_t)stream>>>(
-      (const bf16*)dy, ldy, (const uint8_t*)codes, scale, offsets, work, R, E, N, K, block, nf4 ? 1 : 0);
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return -2;
+  const int planes = eri_linear_4bit_planes(R, N, K, block, offsets != nullptr);
+  if (planes > 65535) return -100;
+  const DgArgs p = {(const bf16*)dy, ldy, (const uint8_t*)codes, scale, offsets, work, R, E, N, K, block};
+  cudaStream_t st = (cudaStream_t)stream;
+  const int code = block % 64 == 0 ? (nf4 ? launch_dg<true, 64>(p, planes, dev, st) : launch_dg<false, 64>(p, planes, dev, st))
+                                   : (nf4 ? launch_dg<true, 32>(p, planes, dev, st) : launch_dg<false, 32>(p, planes, dev, st));
+  if (code) return code;
   const long long vecs = (long long)R * (K / 8);
-  add_planes_kernel<<<(unsigned)((vecs + 255) / 256), 256, 0, (cudaStream_t)stream>>>(work, (bf16*)dx, vecs, planes);
+  add_planes_kernel<<<(unsigned)((vecs + 255) / 256), 256, 0, st>>>(work, (bf16*)dx, vecs, planes);
   return (int)cudaGetLastError();
 }
 

@@ -94,7 +94,7 @@ using torch::autograd::variable_list;
                       int, int, int, int, int, long long, void*))                                                \
   X(eri_linear_4bit, (const void*, long long, const void*, const float*, const int*, const void*, void*, int,    \
                       int, int, int, int, int, void*))                                                           \
-  X(eri_linear_4bit_planes, (int, int, int))                                                                     \
+  X(eri_linear_4bit_planes, (int, int, int, int, int))                                                                   \
   X(eri_linear_4bit_dgrad, (const void*, long long, const void*, const float*, const int*, float*, void*, int,   \
                             int, int, int, int, int, void*))                                                     \
   X(eri_norm_rope_fwd, (const void*, const void*, long long, const void*, const void*, const float*, const float*, \

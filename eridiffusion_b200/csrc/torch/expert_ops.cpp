@@ -188,7 +188,7 @@ struct Linear4bit : torch::autograd::Function<Linear4bit> {
       const Tensor dy = contig(gout[0]);
       dx = empty_bf16({R, K}, dy);
       if (R > 0) {
-        Tensor work = empty_f32({L.eri_linear_4bit_planes(R, N, K), R, K}, dy);
+        Tensor work = empty_f32({L.eri_linear_4bit_planes(R, N, K, (int)m[4], offsets.defined()), R, K}, dy);
         check(L.eri_linear_4bit_dgrad(dy.data_ptr(), N, codes.data_ptr(), (const float*)scale.data_ptr(), ints(offsets),
                                       (float*)work.data_ptr(), dx.data_ptr(), R, E, N, K, (int)m[4], (int)m[5], stream()),
               "linear_4bit_dgrad");

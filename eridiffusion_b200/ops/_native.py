@@ -131,7 +131,7 @@ _SIGNATURES = {
     "eri_expert_gather_bwd": [_P, _L, _P, _L, _P, _P, _P, _P, _P, _I, _I, _I, _I, _P],
     "eri_expert_gemm": [_I, _P, _L, _P, _L, _P, _P, _P, _I, _I, _I, _I, _I, _I, _L, _P],
     "eri_linear_4bit": [_P, _L, _P, _P, _P, _P, _P, _I, _I, _I, _I, _I, _I, _P],
-    "eri_linear_4bit_planes": [_I, _I, _I],
+    "eri_linear_4bit_planes": [_I, _I, _I, _I, _I],
     "eri_linear_4bit_dgrad": [_P, _L, _P, _P, _P, _P, _P, _I, _I, _I, _I, _I, _I, _P],
     "eri_gemv_bf16": [_P, _P, _P, _P, _I, _I, _I, _I, _I, _I, _I, _I, _P],
 }
