@@ -11,7 +11,7 @@
 // and the ragged side on BT columns: kFwd and kDx put BT consecutive rows of one expert on the columns, so an expert of a few
 // rows costs a tile of 32 columns instead of one of 256 lanes, and every tile reads its share of the weights once. kDw puts
 // the K columns of X on the lanes, 256 columns of dY on the columns and reduces over the expert's rows. In all three a
-// lane is the fastest index of the output, so a warp's store of one column is 64 consecutive bytes.
+// lane is the fastest index of the output.
 //
 // Rows of a tile that belong to the next expert are loaded and multiplied but not stored (columns are independent). In kDw
 // the rows are what is summed: the last step of an expert's rows goes through a fix-up warp of each CTA that overwrites the
@@ -37,6 +37,7 @@ constexpr int kMaxExperts = 1024;
 constexpr int BM = 128;         // lanes per CTA (256 per pair)
 constexpr int BK = 64;          // depth of a step
 constexpr int A_BYTES = BM * BK * 2;
+constexpr int kEpi = 16, kEpiBytes = kEpi * BM * 2;      // columns staged by the epilogue at a time, two buffers for each half of the tile
 
 struct ExpertParams {
   const int* offsets;
@@ -54,35 +55,19 @@ struct Cfg {
   static constexpr int kStage = A_BYTES + kB;
   static constexpr int kStages = BT == 256 ? 6 : BT == 128 ? 8 : BT == 64 ? 10 : 11;
   static constexpr int kTmem = 2 * BT;
-  static constexpr int kSmem = kStages * kStage + 1024 + 512;
+  static constexpr int kRing = kStages * kStage + 4 * kEpiBytes;
+  static constexpr int kSmem = kRing + 1024 + 512;
 };
 
-// wait on a barrier that another CTA of the pair arrives on for data in its shared memory
-__device__ __forceinline__ bool mbar_try_wait_cluster(uint64_t* bar, uint32_t parity) {
-  uint32_t ok;
-  asm volatile(
-      "{\n\t.reg .pred P;\n\t"
-      "mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 P, [%1], %2;\n\t"
-      "selp.b32 %0, 1, 0, P;\n\t}\n"
-      : "=r"(ok)
-      : "r"(smem_u32(bar)), "r"(parity)
-      : "memory");
-  return ok != 0;
-}
-__device__ __forceinline__ bool mbar_wait_cluster(uint64_t* bar, uint32_t parity) {
-  if (mbar_try_wait_cluster(bar, parity)) return true;
-  const uint64_t t0 = globaltimer_ns();
-  for (uint32_t i = 0; i < (1u << 26); ++i) {
-    if (mbar_try_wait_cluster(bar, parity)) return true;
-    if ((i & 63u) == 63u && globaltimer_ns() - t0 > ERI_WAIT_LIMIT_NS) return false;
-  }
-  return false;
+__device__ __forceinline__ void named_barrier(int id, int threads) {
+  asm volatile("bar.sync %0, %1;" ::"r"(id), "r"(threads) : "memory");
 }
 
 struct Tile {
   int e, lo, hi;      // expert and the rows of this tile (kDw: all rows of the expert)
   int p0, c0;         // first lane of the pair, first column (kDw)
   int steps;
+  int n;              // columns of the product: the tile's rows rounded up to 32 (kDw: BT)
 };
 
 template <int BT, int MODE>
@@ -101,6 +86,7 @@ struct Sched {
       r.lo = bound[r.e];
       r.hi = bound[r.e + 1];
       r.steps = (r.hi - r.lo + BK - 1) / BK;
+      r.n = BT;
     } else {
       int lo = 0, hi = E;          // before[lo] <= t < before[hi]
       while (hi - lo > 1) {
@@ -114,6 +100,7 @@ struct Sched {
       r.lo = bound[lo] + (i % tt) * BT;
       r.hi = min(r.lo + BT, bound[lo + 1]);
       r.steps = steps;
+      r.n = (r.hi - r.lo + 31) & ~31;
     }
     return r;
   }
@@ -122,17 +109,18 @@ struct Sched {
 template <int BT, int MODE>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(MODE == kDw ? 352 : 320, 1)
 expert_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB,
-                   const __grid_constant__ ExpertParams p) {
+                   const __grid_constant__ CUtensorMap tmB16, const __grid_constant__ ExpertParams p) {
   using C = Cfg<BT>;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-  uint64_t* full = reinterpret_cast<uint64_t*>(smem + C::kStages * C::kStage);
+  uint64_t* full = reinterpret_cast<uint64_t*>(smem + C::kRing);
   uint64_t* empty = full + C::kStages;
   uint64_t* acc_full = empty + C::kStages;
   uint64_t* acc_empty = acc_full + 2;
   uint64_t* tail_full = acc_empty + 2;
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(tail_full + C::kStages);
-  int* bound = reinterpret_cast<int*>(smem + C::kStages * C::kStage + 512);   // [E + 1]
+  uint64_t* tail_done = tail_full + C::kStages;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(tail_done + C::kStages);
+  int* bound = reinterpret_cast<int*>(smem + C::kRing + 512);   // [E + 1]
   int* before = bound + p.E + 1;                                              // [E + 1]
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -141,9 +129,10 @@ expert_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constan
 
   if (threadIdx.x == 0) {
     for (int s = 0; s < C::kStages; ++s) {
-      mbar_init(&full[s], MODE == kDw ? 2 : 1);
+      mbar_init(&full[s], 1);
       mbar_init(&empty[s], 1);
       mbar_init(&tail_full[s], 1);
+      mbar_init(&tail_done[s], 2);           // fix-up warps of both CTAs (used on the leader only)
     }
     for (int b = 0; b < 2; ++b) {
       mbar_init(&acc_full[b], 1);
@@ -225,6 +214,7 @@ expert_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constan
             const int r = tl.lo + k * BK, c0 = tl.c0 + (int)rank * C::kHalf;
             if (r + BK > tl.hi) {          // rows of the next expert come along: this CTA's fix-up warp passes the step on
               uint64_t* tb = &tail_full[stage];
+              if (leader) mbar_arrive(&full[stage]);
               mbar_expect_tx(tb, C::kStage);
               tma_load_2d(sA, &tmA, tb, p0, r);
               tma_load_2d(sA + BK * 128, &tmA, tb, p0 + 64, r);
@@ -232,21 +222,26 @@ expert_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constan
               tma_load_2d(sB + BK * 128, &tmB, tb, c0 + 64, r);
             } else {
               if (leader) mbar_expect_tx(&full[stage], 2 * C::kStage);
-              else mbar_arrive_cluster(bar);
               tma_load_2d_pair(sA, &tmA, bar, p0, r);
               tma_load_2d_pair(sA + BK * 128, &tmA, bar, p0 + 64, r);
               tma_load_2d_pair(sB, &tmB, bar, c0, r);
               tma_load_2d_pair(sB + BK * 128, &tmB, bar, c0 + 64, r);
             }
           } else {
-            if (leader) mbar_expect_tx(&full[stage], 2 * C::kStage);
+            if (leader) mbar_expect_tx(&full[stage], 2 * A_BYTES + tl.n * BK * 2);
             if (MODE == kFwd) {
               tma_load_3d_pair(sA, &tmA, bar, k * BK, p0, tl.e);
             } else {
               tma_load_3d_pair(sA, &tmA, bar, p0, k * BK, tl.e);
               tma_load_3d_pair(sA + BK * 128, &tmA, bar, p0 + 64, k * BK, tl.e);
             }
-            tma_load_2d_pair(sB, &tmB, bar, k * BK, tl.lo + (int)rank * C::kHalf);
+            // a whole tile's half in one copy, a shorter one in groups of 16 rows: what a step takes in is what bounds it
+            const int r = tl.lo + (int)rank * (tl.n >> 1);
+            if (tl.n == BT) {
+              tma_load_2d_pair(sB, &tmB, bar, k * BK, r);
+            } else {
+              for (int i = 0; i < tl.n >> 1; i += 16) tma_load_2d_pair(sB + i * 128, &tmB16, bar, k * BK, r + i);
+            }
           }
           if (++stage == C::kStages) {
             stage = 0;
@@ -258,12 +253,13 @@ expert_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constan
   } else if (warp == 1) {
     if (leader && elect_one()) {
       constexpr bool a_mn = MODE != kFwd, b_mn = MODE == kDw;
-      const uint32_t idesc = umma_idesc_bf16(256, BT, a_mn, b_mn);
       int stage = 0, it = 0;
-      uint32_t phase = 0;
+      uint32_t phase = 0, tails = 0;         // tails: phase of every stage's tail_done
       bool ok = true;
       for (int t = first; ok && t < sched.total; t += stride, ++it) {
-        const int steps = MODE == kDw ? sched.get(t).steps : sched.steps;
+        const Tile tl = sched.get(t);
+        const int steps = tl.steps;
+        const uint32_t idesc = umma_idesc_bf16(256, tl.n, a_mn, b_mn);
         const int buf = it & 1;
         if (!mbar_wait(&acc_empty[buf], ((uint32_t)(it >> 1) & 1) ^ 1)) {
           atomicExch(&g_err, 42);
@@ -272,9 +268,13 @@ expert_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constan
         tc_fence_after();
         const uint32_t d_tmem = tmem_base + buf * BT;
         for (int k = 0; k < steps; ++k) {
-          if (!(MODE == kDw ? mbar_wait_cluster(&full[stage], phase) : mbar_wait(&full[stage], phase))) {
+          ok = mbar_wait(&full[stage], phase);
+          if (MODE == kDw && ok && tl.lo + (k + 1) * BK > tl.hi) {
+            ok = mbar_wait(&tail_done[stage], (tails >> stage) & 1);
+            tails ^= 1u << stage;
+          }
+          if (!ok) {
             atomicExch(&g_err, 43);
-            ok = false;
             break;
           }
           tc_fence_after();
@@ -321,10 +321,11 @@ expert_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constan
         for (int q = 0; q < 4; ++q) *reinterpret_cast<uint4*>(s + q * BK * 128 + rem * 128 + i * 16) = make_uint4(0, 0, 0, 0);
       fence_proxy_async_smem();
       __syncwarp();
-      if (lane == 0) mbar_arrive_cluster(map_to_cta(smem_u32(&full[st]), 0));
+      if (lane == 0) mbar_arrive_cluster(map_to_cta(smem_u32(&tail_done[st]), 0));
     }
   } else {
     const int q = warp & 3, half = (warp - 2) >> 2;
+    bool failed = false;
     if (MODE != kDw) {
       // rows of no expert
       const long long head = (long long)bound[0] * p.P, tail0 = (long long)bound[p.E] * p.P;
@@ -334,39 +335,59 @@ expert_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constan
         *reinterpret_cast<uint4*>(p.out + at) = make_uint4(0, 0, 0, 0);
       }
     }
-    int it = 0;
-    constexpr int W = C::kHalf < 32 ? 16 : 32;       // columns per read of the accumulator
+    // A column of D is 128 consecutive elements of the output per CTA, one per accumulator lane, i.e. per thread: kEpi columns at a
+    // time go through shared memory so that 16 lanes write 256 consecutive bytes. (Two-byte stores straight from the
+    // accumulator, 64 bytes per warp, wrote a gradient of [16, 5120, 2560] at 1.1 TB/s.)
+    uint8_t* stg = smem + C::kStages * C::kStage + half * 2 * kEpiBytes;
+    const int pe = q * 32 + lane;                    // this thread's lane of the CTA
+    const int v_row = q * (kEpi / 4) + (lane >> 4), v_col = (lane & 15) * 8;      // rows v_row, v_row + 2, .. of the staged columns
+    int it = 0, sb = 0;
     for (int t = first; t < sched.total; t += stride, ++it) {
       const Tile tl = sched.get(t);
       const int buf = it & 1;
       if (!mbar_wait(&acc_full[buf], (uint32_t)(it >> 1) & 1)) {
         if (lane == 0) atomicExch(&g_err, 44);
-        break;
+        failed = true;
       }
       tc_fence_after();
-      const int lane_p = tl.p0 + (int)rank * BM + q * 32 + lane;
+      const int p0 = tl.p0 + (int)rank * BM;
       const uint32_t acc = tmem_base + ((uint32_t)(q * 32) << 16) + buf * BT + half * C::kHalf;
-      const bool lane_ok = lane_p < p.P;
-      // columns of this warp's half that are stored, and where the first one goes
+      // columns of this half that are stored, and where the first one goes
       const int col0 = half * C::kHalf;
       const int cols = MODE == kDw ? min(C::kHalf, p.C - tl.c0 - col0) : min(C::kHalf, tl.hi - tl.lo - col0);
-      bf16* o = p.out + (MODE == kDw ? ((long long)tl.e * p.C + tl.c0 + col0) : (long long)(tl.lo + col0)) * p.P + lane_p;
-      for (int c = 0; c < cols; c += W) {
-        uint32_t r[W];
-        if constexpr (W == 32) tmem_ld32(acc + c, r); else tmem_ld16(acc + c, r);
-        tmem_ld_wait();
-        if (lane_ok) {
+      bf16* o = p.out + (MODE == kDw ? ((long long)tl.e * p.C + tl.c0 + col0) : (long long)(tl.lo + col0)) * p.P + p0 + v_col;
+      const bool v_ok = p0 + v_col < p.P && !failed;
+      uint32_t r[kEpi];
+      if (cols > 0) tmem_ld16(acc, r);
+      for (int c = 0; c < cols; c += kEpi, sb ^= 1) {
+        uint8_t* s = stg + sb * kEpiBytes;
+        if (MODE == kDw && p.accum) {                // what the output holds, so that sum and rounding happen once
 #pragma unroll
-          for (int i = 0; i < W; ++i)
-            if (c + i < cols) {
-              bf16* d = o + (long long)(c + i) * p.P;
-              float v = __uint_as_float(r[i]);
-              if (MODE == kDw) {
-                if (tl.steps == 0) v = 0.f;            // no product ran: an expert without rows
-                if (p.accum) v += __bfloat162float(*d);
-              }
-              if (ERI_DBG_RANGE(p.out, p.dbg_out_bytes, d, 2, 81)) *d = __float2bfloat16(v);
-            }
+          for (int i = 0; i < kEpi / 8; ++i)
+            if (v_ok && c + v_row + 2 * i < cols)
+              *reinterpret_cast<uint4*>(s + (v_row + 2 * i) * 256 + v_col * 2) =
+                  *reinterpret_cast<const uint4*>(o + (long long)(c + v_row + 2 * i) * p.P);
+          named_barrier(1 + half, 128);
+        }
+        tmem_ld_wait();
+#pragma unroll
+        for (int i = 0; i < kEpi; ++i) {
+          bf16* d = reinterpret_cast<bf16*>(s + i * 256) + pe;
+          float v = __uint_as_float(r[i]);
+          if (MODE == kDw) {
+            if (tl.steps == 0) v = 0.f;              // no product ran: an expert without rows
+            if (p.accum) v += __bfloat162float(*d);
+          }
+          *d = __float2bfloat16(v);
+        }
+        if (c + kEpi < cols) tmem_ld16(acc + c + kEpi, r);      // under the barrier and the stores
+        named_barrier(1 + half, 128);                // the other buffer's reads are behind every warp that passes
+#pragma unroll
+        for (int i = 0; i < kEpi / 8; ++i) {
+          const int row = c + v_row + 2 * i;
+          bf16* d = o + (long long)row * p.P;
+          if (v_ok && row < cols && ERI_DBG_RANGE(p.out, p.dbg_out_bytes, d, 16, 81))
+            *reinterpret_cast<uint4*>(d) = *reinterpret_cast<const uint4*>(s + (v_row + 2 * i) * 256 + v_col * 2);
         }
       }
       tc_fence_before();
@@ -391,7 +412,7 @@ int num_sms(int dev) {
 }
 
 template <int BT, int MODE>
-int launch(const CUtensorMap& ta, const CUtensorMap& tb, const ExpertParams& p, long long tiles, int dev, cudaStream_t st) {
+int launch(const CUtensorMap& ta, const CUtensorMap& tb, const CUtensorMap& tb16, const ExpertParams& p, long long tiles, int dev, cudaStream_t st) {
   constexpr int kMost = Cfg<BT>::kSmem + 2 * (kMaxExperts + 1) * (int)sizeof(int);
   static_assert(kMost <= 232448, "shared memory of a CTA");
   static bool configured[64] = {};
@@ -403,7 +424,7 @@ int launch(const CUtensorMap& ta, const CUtensorMap& tb, const ExpertParams& p, 
   const int smem = Cfg<BT>::kSmem + 2 * (p.E + 1) * (int)sizeof(int);
   const int pairs = num_sms(dev) / 2;
   const int grid = (int)(tiles < pairs ? (tiles < 1 ? 1 : tiles) : pairs);
-  expert_gemm_kernel<BT, MODE><<<grid * 2, MODE == kDw ? 352 : 320, smem, st>>>(ta, tb, p);
+  expert_gemm_kernel<BT, MODE><<<grid * 2, MODE == kDw ? 352 : 320, smem, st>>>(ta, tb, tb16, p);
   return (int)cudaGetLastError();
 }
 
@@ -421,8 +442,9 @@ int map3(CUtensorMap* m, const void* ptr, int K, int N, int E, int box_rows) {
 }
 
 template <int BT>
-int run_rows(int mode, const CUtensorMap& ta, const CUtensorMap& tb, const ExpertParams& p, long long tiles, int dev, cudaStream_t st) {
-  return mode == kFwd ? launch<BT, kFwd>(ta, tb, p, tiles, dev, st) : launch<BT, kDx>(ta, tb, p, tiles, dev, st);
+int run_rows(int mode, const CUtensorMap& ta, const CUtensorMap& tb, const CUtensorMap& tb16, const ExpertParams& p, long long tiles,
+             int dev, cudaStream_t st) {
+  return mode == kFwd ? launch<BT, kFwd>(ta, tb, tb16, p, tiles, dev, st) : launch<BT, kDx>(ta, tb, tb16, p, tiles, dev, st);
 }
 
 }  // namespace
@@ -453,12 +475,12 @@ int eri_expert_gemm(int mode, const void* rows, long long ld_rows, const void* r
   p.P = mode == kFwd ? N : K;
   p.C = mode == kFwd ? K : N;
   const long long num_p = (p.P + 2 * BM - 1) / (2 * BM);
-  CUtensorMap ta, tb;
+  CUtensorMap ta, tb, tb16;
   if (mode == kDw) {
     if (map2(&ta, rows, K, R, ld_rows, BK) || map2(&tb, rows2, N, R, ld_rows2, BK)) return -20;
     const long long tiles = (long long)E * num_p * ((N + 255) / 256);
     if (tiles > 0x7fffffff) return -3;
-    return launch<256, kDw>(ta, tb, p, tiles, dev, st);
+    return launch<256, kDw>(ta, tb, tb, p, tiles, dev, st);
   }
   int bt = columns;
   if (!bt) {
@@ -469,12 +491,14 @@ int eri_expert_gemm(int mode, const void* rows, long long ld_rows, const void* r
   // each expert starts a tile of its own: at most R / bt full ones and one partial tile per expert that has rows
   const long long tiles = ((long long)R / bt + (E < R ? E : R)) * num_p;
   if (tiles > 0x7fffffff) return -3;
-  if (map3(&ta, w, K, N, E, mode == kFwd ? BM : BK) || map2(&tb, rows, mode == kFwd ? K : N, R, ld_rows, bt / 2)) return -20;
+  if (map3(&ta, w, K, N, E, mode == kFwd ? BM : BK) || map2(&tb, rows, mode == kFwd ? K : N, R, ld_rows, bt / 2) ||
+      map2(&tb16, rows, mode == kFwd ? K : N, R, ld_rows, 16))
+    return -20;
   switch (bt) {
-    case 32: return run_rows<32>(mode, ta, tb, p, tiles, dev, st);
-    case 64: return run_rows<64>(mode, ta, tb, p, tiles, dev, st);
-    case 128: return run_rows<128>(mode, ta, tb, p, tiles, dev, st);
-    default: return run_rows<256>(mode, ta, tb, p, tiles, dev, st);
+    case 32: return run_rows<32>(mode, ta, tb, tb16, p, tiles, dev, st);
+    case 64: return run_rows<64>(mode, ta, tb, tb16, p, tiles, dev, st);
+    case 128: return run_rows<128>(mode, ta, tb, tb16, p, tiles, dev, st);
+    default: return run_rows<256>(mode, ta, tb, tb16, p, tiles, dev, st);
   }
 }
 

@@ -336,3 +336,24 @@ def test_on_another_stream():
         y = F.expert_linear(late, w, off)
     side.synchronize()
     assert torch.equal(y, ref)
+
+
+def test_first_call_of_a_thread():
+    """Operand maps are encoded by the driver, which wants a context of the calling thread; a new thread has none yet."""
+    import threading
+    g = _gen(15)
+    x, w, off = _mk(g, 48, 88), _mk(g, 2, 40, 88, std=0.1), _offsets([20, 28])
+    ref = F.expert_linear(x, w, off)
+    x2, w2 = x.clone(), w.clone()               # other addresses: nothing of theirs is encoded yet
+    torch.cuda.synchronize()
+    got = []
+
+    def call():
+        try:
+            got.append(F.expert_linear(x2, w2, off))
+        except RuntimeError as e:
+            got.append(e)
+    t = threading.Thread(target=call)
+    t.start(), t.join()
+    torch.cuda.synchronize()
+    assert torch.is_tensor(got[0]) and torch.equal(got[0], ref), got[0]
