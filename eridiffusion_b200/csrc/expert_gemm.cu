@@ -37,7 +37,9 @@ constexpr int kMaxExperts = 1024;
 constexpr int BM = 128;         // lanes per CTA (256 per pair)
 constexpr int BK = 64;          // depth of a step
 constexpr int A_BYTES = BM * BK * 2;
-constexpr int kEpi = 16, kEpiBytes = kEpi * BM * 2;      // columns staged by the epilogue at a time, two buffers for each half of the tile
+// The epilogue stages kEpi columns of 128 lanes at a time, two buffers for each half of the tile. Rows of 272 bytes: the eight 16-byte
+// rows that a matrix store touches lie in different banks.
+constexpr int kEpi = 16, kEpiPitch = BM * 2 + 16, kEpiBytes = kEpi * kEpiPitch;
 
 struct ExpertParams {
   const int* offsets;
@@ -59,6 +61,23 @@ struct Cfg {
   static constexpr int kSmem = kRing + 1024 + 512;
 };
 
+// 16 accumulator lanes x 16 columns: thread i gets lanes i / 4 (r[0], r[1], r[4], r[5]) and i / 4 + 8, columns 2 (i % 4) + {0, 1} and 8 more.
+__device__ __forceinline__ void tmem_ld_16x16(uint32_t taddr, uint32_t (&r)[8]) {
+  asm volatile("tcgen05.ld.sync.aligned.16x256b.x2.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7])
+               : "r"(taddr)
+               : "memory");
+}
+// Four 8 x 8 blocks between registers (two neighbouring columns each) and shared memory, transposed: a row there is a column here.
+__device__ __forceinline__ void store_blocks_t(uint32_t addr, uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
+  asm volatile("stmatrix.sync.aligned.m8n8.x4.trans.shared.b16 [%0], {%1,%2,%3,%4};" ::"r"(addr), "r"(a), "r"(b), "r"(c), "r"(d) : "memory");
+}
+__device__ __forceinline__ void load_blocks_t(uint32_t addr, uint32_t (&v)[4]) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];"
+               : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3])
+               : "r"(addr)
+               : "memory");
+}
 __device__ __forceinline__ void named_barrier(int id, int threads) {
   asm volatile("bar.sync %0, %1;" ::"r"(id), "r"(threads) : "memory");
 }
@@ -335,11 +354,12 @@ expert_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constan
         *reinterpret_cast<uint4*>(p.out + at) = make_uint4(0, 0, 0, 0);
       }
     }
-    // A column of D is 128 consecutive elements of the output per CTA, one per accumulator lane, i.e. per thread: kEpi columns at a
-    // time go through shared memory so that 16 lanes write 256 consecutive bytes. (Two-byte stores straight from the
-    // accumulator, 64 bytes per warp, wrote a gradient of [16, 5120, 2560] at 1.1 TB/s.)
+    // A column of D is 128 consecutive elements of the output per CTA, one per accumulator lane: kEpi columns at a time are transposed
+    // through shared memory (eight 8 x 8 blocks per warp, two matrix stores) so that 16 lanes write 256 consecutive bytes.
+    // Two-byte stores straight from the accumulator, 64 bytes per warp, wrote a gradient of [16, 5120, 2560] at 1.1 TB/s.
     uint8_t* stg = smem + C::kStages * C::kStage + half * 2 * kEpiBytes;
-    const int pe = q * 32 + lane;                    // this thread's lane of the CTA
+    // matrix i of a store is given by lanes 8 i .. 8 i + 7: columns 8 (i / 2) + .., lanes 8 (i % 2) + .. of a half of the quadrant
+    const uint32_t m_off = (uint32_t)(((lane >> 4) * 8 + (lane & 7)) * kEpiPitch + (q * 32 + ((lane >> 3) & 1) * 8) * 2);
     const int v_row = q * (kEpi / 4) + (lane >> 4), v_col = (lane & 15) * 8;      // rows v_row, v_row + 2, .. of the staged columns
     int it = 0, sb = 0;
     for (int t = first; t < sched.total; t += stride, ++it) {
@@ -357,37 +377,51 @@ expert_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constan
       const int cols = MODE == kDw ? min(C::kHalf, p.C - tl.c0 - col0) : min(C::kHalf, tl.hi - tl.lo - col0);
       bf16* o = p.out + (MODE == kDw ? ((long long)tl.e * p.C + tl.c0 + col0) : (long long)(tl.lo + col0)) * p.P + p0 + v_col;
       const bool v_ok = p0 + v_col < p.P && !failed;
-      uint32_t r[kEpi];
-      if (cols > 0) tmem_ld16(acc, r);
+      uint32_t r[2][8];                              // the two halves of the quadrant
+      if (cols > 0) {
+        tmem_ld_16x16(acc, r[0]);
+        tmem_ld_16x16(acc + (16u << 16), r[1]);
+      }
       for (int c = 0; c < cols; c += kEpi, sb ^= 1) {
         uint8_t* s = stg + sb * kEpiBytes;
+        const uint32_t s_m = smem_u32(s) + m_off;
         if (MODE == kDw && p.accum) {                // what the output holds, so that sum and rounding happen once
 #pragma unroll
           for (int i = 0; i < kEpi / 8; ++i)
             if (v_ok && c + v_row + 2 * i < cols)
-              *reinterpret_cast<uint4*>(s + (v_row + 2 * i) * 256 + v_col * 2) =
+              *reinterpret_cast<uint4*>(s + (v_row + 2 * i) * kEpiPitch + v_col * 2) =
                   *reinterpret_cast<const uint4*>(o + (long long)(c + v_row + 2 * i) * p.P);
           named_barrier(1 + half, 128);
         }
         tmem_ld_wait();
 #pragma unroll
-        for (int i = 0; i < kEpi; ++i) {
-          bf16* d = reinterpret_cast<bf16*>(s + i * 256) + pe;
-          float v = __uint_as_float(r[i]);
-          if (MODE == kDw) {
-            if (tl.steps == 0) v = 0.f;              // no product ran: an expert without rows
-            if (p.accum) v += __bfloat162float(*d);
+        for (int h = 0; h < 2; ++h) {
+          float f[8];
+#pragma unroll
+          for (int i = 0; i < 8; ++i) f[i] = MODE == kDw && tl.steps == 0 ? 0.f : __uint_as_float(r[h][i]);     // (an expert without rows)
+          if (MODE == kDw && p.accum) {
+            uint32_t old[4];
+            load_blocks_t(s_m + h * 32, old);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              const float2 b = bf162_bits_to_float2(old[i]);
+              f[2 * i] += b.x;
+              f[2 * i + 1] += b.y;
+            }
           }
-          *d = __float2bfloat16(v);
+          store_blocks_t(s_m + h * 32, pack_bf162(f[0], f[1]), pack_bf162(f[2], f[3]), pack_bf162(f[4], f[5]), pack_bf162(f[6], f[7]));
         }
-        if (c + kEpi < cols) tmem_ld16(acc + c + kEpi, r);      // under the barrier and the stores
+        if (c + kEpi < cols) {                       // the next columns, under the barrier and the stores
+          tmem_ld_16x16(acc + c + kEpi, r[0]);
+          tmem_ld_16x16(acc + c + kEpi + (16u << 16), r[1]);
+        }
         named_barrier(1 + half, 128);                // the other buffer's reads are behind every warp that passes
 #pragma unroll
         for (int i = 0; i < kEpi / 8; ++i) {
           const int row = c + v_row + 2 * i;
           bf16* d = o + (long long)row * p.P;
           if (v_ok && row < cols && ERI_DBG_RANGE(p.out, p.dbg_out_bytes, d, 16, 81))
-            *reinterpret_cast<uint4*>(d) = *reinterpret_cast<const uint4*>(s + (v_row + 2 * i) * 256 + v_col * 2);
+            *reinterpret_cast<uint4*>(d) = *reinterpret_cast<const uint4*>(s + (v_row + 2 * i) * kEpiPitch + v_col * 2);
         }
       }
       tc_fence_before();
@@ -484,8 +518,13 @@ int eri_expert_gemm(int mode, const void* rows, long long ld_rows, const void* r
   }
   int bt = columns;
   if (!bt) {
+    // Rows of an expert on average against the tile's columns. A short tile multiplies and loads only its rows, so a tall one costs
+    // little there; it has fewer stages in flight, a low one reads the weights once more per tile. us, forward / dX, 16
+    // experts, 4096 x 2048 (first row 5120 x 2560):  32 | 64 | 128 | 256 columns
+    //   4 rows    64.5/68.8 | 66.3/70.9 | 68.0/72.5 | 70.4/73.6       64 rows   61.0/65.0 | 53.0/50.9 | 48.9/46.7 | 51.1/47.0
+    //   32 rows   47.2/50.4 | 48.1/46.0 | 47.5/45.4 | 49.7/45.4       128 rows  97.3/95.2 | 67.9/69.9 | 57.6/55.5 | 54.9/52.0
     const int per = R / E;
-    bt = per <= 32 ? 32 : per <= 64 ? 64 : per <= 128 ? 128 : 256;
+    bt = per <= 8 ? 32 : per <= 16 ? 64 : per <= 96 ? 128 : 256;
   }
   if (bt != 32 && bt != 64 && bt != 128 && bt != 256) return -4;
   // each expert starts a tile of its own: at most R / bt full ones and one partial tile per expert that has rows
