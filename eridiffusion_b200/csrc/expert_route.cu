@@ -180,12 +180,36 @@ __global__ void __launch_bounds__(256) route_bwd_kernel(const T* __restrict__ sc
 // Stable counting sort by one cluster (one to eight CTAs of 32 warps). Every warp owns a consecutive piece of the choices and a
 // private row of counters in shared memory: (1) it counts its piece, (2) the counters become prefix sums over the warps of a
 // CTA, (3) the CTAs' totals are added over distributed shared memory, (4) the warp walks its piece again and hands out
-// positions. Equal experts inside one group of 32 are ranked by the lanes below, so the order is that of the choices.
-constexpr int kPlanThreads = 1024, kPlanWarps = kPlanThreads / 32;
+// positions. Equal experts inside one group of 32 are found by ballots and ranked by the lanes below, so the order is that of the
+// choices. A piece of at most kHold groups stays in registers between the two walks.
+// Bound by latency: two rounds of loads, four barriers, one read of remote totals. 49152 choices, 64 experts: see kernel table.
+constexpr int kPlanThreads = 1024, kPlanWarps = kPlanThreads / 32, kHold = 8, kMaxCtas = 8;
 
 __device__ __forceinline__ int load_choice(const void* idx, int wide, long long i, int E) {
   const long long e = wide ? reinterpret_cast<const long long*>(idx)[i] : (long long)reinterpret_cast<const int*>(idx)[i];
   return e >= 0 && e < E ? (int)e : -1;
+}
+__device__ __forceinline__ void load_group(int (&c)[kHold], const void* idx, int wide, long long i0, long long hi, int lane, int E) {
+#pragma unroll
+  for (int u = 0; u < kHold; ++u) {
+    const long long i = i0 + 32 * u + lane;
+    c[u] = i < hi ? load_choice(idx, wide, i, E) : -1;
+  }
+}
+// Lanes of the warp whose choice is c's (one ballot per bit of an expert's number; lanes without a choice are nobody's).
+__device__ __forceinline__ unsigned same_choice(int c, int bits) {
+  unsigned m = __ballot_sync(0xffffffffu, c >= 0);
+  for (int b = 0; b < bits; ++b) {
+    const bool on = (c >> b) & 1;
+    const unsigned v = __ballot_sync(0xffffffffu, on);
+    m &= on ? v : ~v;
+  }
+  return m;
+}
+__device__ __forceinline__ int ld_cluster(uint32_t addr) {      // not ordered against other loads: all of a thread's are in flight
+  int v;
+  asm("ld.shared::cluster.u32 %0, [%1];" : "=r"(v) : "r"(addr));
+  return v;
 }
 
 __global__ void __launch_bounds__(kPlanThreads) expert_plan_kernel(const void* __restrict__ idx, int wide, int n, int E, int ctas,
@@ -193,8 +217,9 @@ __global__ void __launch_bounds__(kPlanThreads) expert_plan_kernel(const void* _
                                                                    int* __restrict__ source) {
   extern __shared__ int plan_smem[];
   int* total = plan_smem;                 // [E] this CTA's choices of every expert
-  int* base = total + E;                  // [E] first row of this CTA's choices of every expert
-  int* cnt = base + E;                    // [kPlanWarps][E]
+  int* base = total + E;                  // [E] rows of lower CTAs of the expert
+  int* first = base + E;                  // [E] first row of the expert
+  int* cnt = first + E;                   // [kPlanWarps][E]
   __shared__ int s_live;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int rank = ctas > 1 ? (int)cluster_ctarank() : 0;
@@ -202,25 +227,27 @@ __global__ void __launch_bounds__(kPlanThreads) expert_plan_kernel(const void* _
   const long long piece = (((long long)n + warps - 1) / warps + 31) / 32 * 32;
   const long long lo = min((long long)(rank * kPlanWarps + warp) * piece, (long long)n), hi = min(lo + piece, (long long)n);
   int* mine = cnt + (size_t)warp * E;
+  const int bits = 32 - __clz(E - 1);
+  int c[kHold];
+  unsigned same[kHold];
+  load_group(c, idx, wide, lo, hi, lane, E);
   for (int e = lane; e < E; e += 32) mine[e] = 0;
   __syncwarp();
-  for (long long i0 = lo; i0 < hi; i0 += 128) {       // four loads in flight
-    int c[4];
+  for (long long i0 = lo; i0 < hi; i0 += 32 * kHold) {
+    if (i0 != lo) load_group(c, idx, wide, i0, hi, lane, E);
 #pragma unroll
-    for (int u = 0; u < 4; ++u) {
-      const long long i = i0 + 32 * u + lane;
-      c[u] = i < hi ? load_choice(idx, wide, i, E) : -1;
-    }
-#pragma unroll
-    for (int u = 0; u < 4; ++u) {
-      const unsigned same = __match_any_sync(0xffffffffu, c[u]);
-      if (c[u] >= 0 && lane == __ffs(same) - 1) mine[c[u]] += __popc(same);
-      __syncwarp();
+    for (int u = 0; u < kHold; ++u) {
+      if (i0 + 32 * u < hi) {
+        same[u] = same_choice(c[u], bits);
+        if (c[u] >= 0 && lane == __ffs(same[u]) - 1) mine[c[u]] += __popc(same[u]);
+        __syncwarp();
+      }
     }
   }
   __syncthreads();
   for (int e = threadIdx.x; e < E; e += kPlanThreads) {
     int sum = 0;
+#pragma unroll 8
     for (int q = 0; q < kPlanWarps; ++q) {
       const int here = cnt[(size_t)q * E + e];
       cnt[(size_t)q * E + e] = sum;
@@ -228,20 +255,32 @@ __global__ void __launch_bounds__(kPlanThreads) expert_plan_kernel(const void* _
     }
     total[e] = sum;
   }
+  if (ctas > 1) cluster_sync_all(); else __syncthreads();
+  // every CTA adds up all totals itself
+  for (int e = threadIdx.x; e < E; e += kPlanThreads) {
+    int before = 0, all = 0;
+    if (ctas > 1) {
+      int x[kMaxCtas];
+#pragma unroll
+      for (int q = 0; q < kMaxCtas; ++q) x[q] = q < ctas ? ld_cluster(map_to_cta(smem_u32(total + e), (uint32_t)q)) : 0;
+#pragma unroll
+      for (int q = 0; q < kMaxCtas; ++q) {
+        all += x[q];
+        before += q < rank ? x[q] : 0;
+      }
+    } else {
+      all = total[e];
+    }
+    first[e] = all;
+    base[e] = before;
+  }
+  // no CTA leaves while another may read its totals: the wait is at the end
+  if (ctas > 1) asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
   __syncthreads();
-  if (ctas > 1) cluster_sync_all();
-  // every CTA adds up all totals itself: base[e] = rows of lower experts + rows of e in lower CTAs
   if (warp == 0) {
     int run = 0;
     for (int e0 = 0; e0 < E; e0 += 32) {
-      const int e = e0 + lane;
-      int before = 0, all = 0;
-      if (e < E)
-        for (int c = 0; c < ctas; ++c) {
-          const int x = ctas > 1 ? __float_as_int(ld_shared_cluster_f32(map_to_cta(smem_u32(total + e), (uint32_t)c))) : total[e];
-          all += x;
-          before += c < rank ? x : 0;
-        }
+      const int e = e0 + lane, all = e < E ? first[e] : 0;
       int scan = all;
 #pragma unroll
       for (int o = 1; o < 32; o <<= 1) {
@@ -249,7 +288,7 @@ __global__ void __launch_bounds__(kPlanThreads) expert_plan_kernel(const void* _
         if (lane >= o) scan += up;
       }
       if (e < E) {
-        base[e] = run + scan - all + before;
+        first[e] = run + scan - all;
         if (rank == 0) offsets[e] = run + scan - all;
       }
       run += __shfl_sync(0xffffffffu, scan, 31);
@@ -260,30 +299,28 @@ __global__ void __launch_bounds__(kPlanThreads) expert_plan_kernel(const void* _
     }
   }
   __syncthreads();
-  if (ctas > 1) cluster_sync_all();       // no CTA leaves while another may read its totals
-  for (long long i0 = lo; i0 < hi; i0 += 128) {
-    int c[4];
+  const bool held = piece <= 32 * kHold;
+  for (long long i0 = lo; i0 < hi; i0 += 32 * kHold) {
+    if (!held) load_group(c, idx, wide, i0, hi, lane, E);
 #pragma unroll
-    for (int u = 0; u < 4; ++u) {
-      const long long i = i0 + 32 * u + lane;
-      c[u] = i < hi ? load_choice(idx, wide, i, E) : -1;
-    }
-#pragma unroll
-    for (int u = 0; u < 4; ++u) {
-      const long long i = i0 + 32 * u + lane;
-      const unsigned same = __match_any_sync(0xffffffffu, c[u]);
-      int pos = -1;
-      if (c[u] >= 0) pos = base[c[u]] + mine[c[u]] + __popc(same & ((1u << lane) - 1u));
-      __syncwarp();
-      if (c[u] >= 0 && lane == __ffs(same) - 1) mine[c[u]] += __popc(same);
-      __syncwarp();
-      if (i < hi) {
-        rows[i] = pos;
-        if (pos >= 0 && ERI_DBG_INDEX(pos, n, 71)) source[pos] = (int)i;
+    for (int u = 0; u < kHold; ++u) {
+      if (i0 + 32 * u < hi) {
+        const long long i = i0 + 32 * u + lane;
+        if (!held) same[u] = same_choice(c[u], bits);
+        int pos = -1;
+        if (c[u] >= 0) pos = first[c[u]] + base[c[u]] + mine[c[u]] + __popc(same[u] & ((1u << lane) - 1u));
+        __syncwarp();
+        if (c[u] >= 0 && lane == __ffs(same[u]) - 1) mine[c[u]] += __popc(same[u]);
+        __syncwarp();
+        if (i < hi) {
+          rows[i] = pos;
+          if (pos >= 0 && ERI_DBG_INDEX(pos, n, 71)) source[pos] = (int)i;
+        }
       }
     }
   }
   for (long long i = (long long)s_live + rank * kPlanThreads + threadIdx.x; i < n; i += (long long)ctas * kPlanThreads) source[i] = -1;
+  if (ctas > 1) asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
 
 // ------------------------------------------------------------------------------------------- copies
@@ -309,40 +346,56 @@ __global__ void __launch_bounds__(256) expert_scatter_kernel(const bf16* __restr
     *reinterpret_cast<bf16x8*>(xs + (long long)from * D + it * 8) = z;
 }
 
-// out[t] = sum_j w[t, j] y[rows[t, j]] in 32 bits and ascending j, rounded once. Up to four rows of y are in flight per thread.
+// out[t] = sum_j w[t, j] y[rows[t, j]] in 32 bits and ascending j, rounded once. A warp owns 512 columns of one token, a lane twice
+// eight of them: the token's rows and weights are loaded once per warp and handed round, and eight loads of y are in flight per lane.
+constexpr int kFly = 4, kGatherCols = 512;
 __global__ void __launch_bounds__(256) expert_gather_kernel(const bf16* __restrict__ y, long long ldy, const int* __restrict__ rows,
                                                             const float* __restrict__ w, bf16* __restrict__ out, long long items,
-                                                            int vecs, int k, int n_rows, int D) {
-  const long long stride = (long long)gridDim.x * blockDim.x;
-  for (long long it = (long long)blockIdx.x * blockDim.x + threadIdx.x; it < items; it += stride) {
-    const long long t = it / vecs;
-    const int c = (int)(it - t * vecs) * 8;
-    float acc[8];
+                                                            int chunks, int k, int n_rows, int D) {
+  const int lane = threadIdx.x & 31;
+  const long long stride = (long long)gridDim.x * (blockDim.x >> 5);
+  for (long long it = (long long)blockIdx.x * (blockDim.x >> 5) + (threadIdx.x >> 5); it < items; it += stride) {
+    const long long t = it / chunks;
+    const int c = (int)(it - t * chunks) * kGatherCols + lane * 8;
+    const bool on0 = c < D, on1 = c + 256 < D;
+    float acc[2][8];
 #pragma unroll
-    for (int q = 0; q < 8; ++q) acc[q] = 0.f;
-    for (int j0 = 0; j0 < k; j0 += 4) {
-      bf16x8 v[4];
-      float f[4];
-      bool on[4];
-#pragma unroll
-      for (int u = 0; u < 4; ++u) {
-        const int r = j0 + u < k ? rows[t * k + j0 + u] : -1;
-        on[u] = r >= 0 && r < n_rows;
-        if (on[u]) {
-          v[u] = *reinterpret_cast<const bf16x8*>(y + (long long)r * ldy + c);
-          f[u] = w ? w[t * k + j0 + u] : 1.f;
-        }
+    for (int q = 0; q < 8; ++q) acc[0][q] = acc[1][q] = 0.f;
+    for (int j0 = 0; j0 < k; j0 += 32) {
+      int r = -1;
+      float f = 1.f;
+      if (j0 + lane < k) {
+        r = rows[t * k + j0 + lane];
+        if (w) f = w[t * k + j0 + lane];
+        if (r >= n_rows) r = -1;
       }
+      const int here = min(32, k - j0);
+      for (int j = 0; j < here; j += kFly) {
+        bf16x8 v[kFly][2];
+        int ru[kFly];
 #pragma unroll
-      for (int u = 0; u < 4; ++u)
-        if (on[u]) {
-          float a[8];
-          unpack8(v[u], a);
-#pragma unroll
-          for (int q = 0; q < 8; ++q) acc[q] = fmaf(f[u], a[q], acc[q]);
+        for (int u = 0; u < kFly; ++u) {
+          ru[u] = j + u < here ? __shfl_sync(0xffffffffu, r, j + u) : -1;
+          const bf16* src = y + (long long)ru[u] * ldy + c;
+          if (ru[u] >= 0 && on0) v[u][0] = *reinterpret_cast<const bf16x8*>(src);
+          if (ru[u] >= 0 && on1) v[u][1] = *reinterpret_cast<const bf16x8*>(src + 256);
         }
+#pragma unroll
+        for (int u = 0; u < kFly; ++u)
+          if (ru[u] >= 0) {
+            const float fu = __shfl_sync(0xffffffffu, f, j + u);
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+              float a[8];
+              unpack8(v[u][h], a);
+#pragma unroll
+              for (int q = 0; q < 8; ++q) acc[h][q] = fmaf(fu, a[q], acc[h][q]);
+            }
+          }
+      }
     }
-    *reinterpret_cast<bf16x8*>(out + t * D + c) = pack8(acc);
+    if (on0) *reinterpret_cast<bf16x8*>(out + t * D + c) = pack8(acc[0]);
+    if (on1) *reinterpret_cast<bf16x8*>(out + t * D + c + 256) = pack8(acc[1]);
   }
 }
 
@@ -451,10 +504,9 @@ int route_bwd(const void* s, long long ld, const void* allowed, const long long*
   return (int)cudaGetLastError();
 }
 
-// CTAs for `items` threads of work: at most what keeps every SM's 2048 threads busy eight times over, the kernels loop beyond.
-unsigned copy_grid(long long items) {
+unsigned copy_grid(long long items) {       // a thread per item; the kernels loop beyond what a grid holds
   const long long g = (items + 255) / 256;
-  return (unsigned)(g < 1 ? 1 : g > 148 * 64 ? 148 * 64 : g);
+  return (unsigned)(g > 0x7fffffff ? 0x7fffffff : g);
 }
 
 bool dims_ok(int tokens, int k, int n_rows, int D) { return tokens >= 1 && k >= 1 && n_rows >= 0 && D >= 8 && D % 8 == 0; }
@@ -484,18 +536,17 @@ int eri_expert_route_bwd(const void* scores, long long ld, const void* allowed, 
 // idx: n choices (int64 when wide, else int32). offsets [E + 1], rows [n], source [n] int32.
 int eri_expert_plan(const void* idx, int wide, int n, int E, int* offsets, int* rows, int* source, void* stream) {
   if (n < 0 || E < 1 || E > kMaxExperts) return -1;
-  const int smem = (kPlanWarps + 2) * E * (int)sizeof(int);
+  const int smem = (kPlanWarps + 3) * E * (int)sizeof(int);
   int dev = 0;
   if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return -2;
   static bool configured[64] = {};
   if (!configured[dev]) {
     if (cudaFuncSetAttribute(expert_plan_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                             (kPlanWarps + 2) * kMaxExperts * (int)sizeof(int)) != cudaSuccess)
+                             (kPlanWarps + 3) * kMaxExperts * (int)sizeof(int)) != cudaSuccess)
       return -3;
     configured[dev] = true;
   }
-  // a warp reads 128 choices at a time: more CTAs only when one would loop
-  const int ctas = n <= 4096 ? 1 : n <= 8192 ? 2 : n <= 16384 ? 4 : 8;
+  const int ctas = n <= 4096 ? 1 : n <= 8192 ? 2 : n <= 16384 ? 4 : kMaxCtas;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(ctas);
   cfg.blockDim = dim3(kPlanThreads);
@@ -522,9 +573,10 @@ int eri_expert_scatter(const void* x, long long ldx, const int* rows, const int*
 int eri_expert_gather(const void* y, long long ldy, const int* rows, const float* w, void* out, int tokens, int k, int n_rows, int D,
                       void* stream) {
   if (!dims_ok(tokens, k, n_rows, D) || ldy % 8 || (((uintptr_t)y | (uintptr_t)out) & 15)) return -1;
-  const long long items = (long long)tokens * (D / 8);
-  expert_gather_kernel<<<copy_grid(items), 256, 0, (cudaStream_t)stream>>>((const bf16*)y, ldy, rows, w, (bf16*)out, items, D / 8, k,
-                                                                           n_rows, D);
+  const int chunks = (D + kGatherCols - 1) / kGatherCols;
+  const long long items = (long long)tokens * chunks;
+  expert_gather_kernel<<<copy_grid(items * 32), 256, 0, (cudaStream_t)stream>>>((const bf16*)y, ldy, rows, w, (bf16*)out, items, chunks,
+                                                                                k, n_rows, D);
   return (int)cudaGetLastError();
 }
 
