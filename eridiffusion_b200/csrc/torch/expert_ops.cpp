@@ -185,7 +185,7 @@ struct Linear4bit : torch::autograd::Function<Linear4bit> {
     const CUDAGuard guard(codes.device());
     Tensor dx, db;
     if (ctx->needs_input_grad(0)) {
-      const Tensor dy = contig(gout[0]);
+      const Tensor dy = contig16(gout[0]);
       dx = empty_bf16({R, K}, dy);
       if (R > 0) {
         Tensor work = empty_f32({L.eri_linear_4bit_planes(R, N, K, (int)m[4], offsets.defined()), R, K}, dy);

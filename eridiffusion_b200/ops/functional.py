@@ -1069,7 +1069,7 @@ def linear_4bit(x, q, offsets=None, bias=None):
         raise ValueError(f"linear_4bit: bias {tuple(bias.shape)} for {Nn} outputs")
     _same_device("linear_4bit", x, q.data, q.scale, bias)
     rows = x.numel() // K
-    if _native_ok(x, bias) and rows <= (_CODES_EXPERT_ROWS if experts else _CODES_ROWS) and K % q.block == 0 and q.block % 32 == 0 \
+    if _native_ok(x, bias) and rows <= (_CODES_EXPERT_ROWS if experts else _CODES_ROWS) and E <= _MAX_EXPERTS and K % q.block == 0 and q.block % 32 == 0 \
             and q.data.is_contiguous() and q.data.data_ptr() % 16 == 0 and Nn > 0:
         y = N.ops().linear_4bit(x.reshape(rows, K), q.data, q.scale.float().contiguous(),
                                 None if offsets is None else offsets.to(torch.int32).contiguous(), bias, E, Nn, q.block, q.kind == "nf4")
