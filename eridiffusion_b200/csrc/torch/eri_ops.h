@@ -230,8 +230,8 @@ std::vector<Tensor> expert_plan(const Tensor& idx, int64_t experts);
 Tensor expert_dispatch(const Tensor& x, const Tensor& rows, const Tensor& offsets);
 Tensor expert_combine(const Tensor& y, const Tensor& w, const Tensor& rows, const Tensor& offsets);
 Tensor expert_linear(const Tensor& x, const Tensor& w, const Tensor& offsets, int64_t columns, bool accum);
-Tensor linear_4bit(const Tensor& x, const Tensor& codes, const Tensor& scale, const OptT& offsets, const OptT& bias, int64_t experts,
-                   int64_t N, int64_t block, bool nf4);
+OptT linear_4bit(const Tensor& x, const Tensor& codes, const Tensor& scale, const OptT& offsets, const OptT& bias, int64_t experts,
+                 int64_t N, int64_t block, bool nf4);
 
 // Optional tensors among a node's arguments. Function::apply takes them as std::optional, and only the present ones
 // get an edge: ``Args`` records which are present (arguments come first, in order) so that the backward can ask

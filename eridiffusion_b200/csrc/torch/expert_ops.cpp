@@ -202,9 +202,19 @@ struct Linear4bit : torch::autograd::Function<Linear4bit> {
 
 }  // namespace
 
-std::vector<Tensor> expert_route(const Tensor& scores, const OptT& allowed, int64_t k, bool normalize) {
-  if (any_grad({&scores})) return ExpertRoute::apply(scores, allowed, k, normalize);
-  return ExpertRoute::forward(nullptr, scores, allowed, k, normalize);
+namespace {
+void same_device(const char* what, const Tensor& a, std::initializer_list<const Tensor*> ts) {
+  for (const Tensor* t : ts)
+    TORCH_CHECK_VALUE(!t->defined() || t->device() == a.device(), what, ": tensors on different devices: ", a.device(), " and ", t->device());
+}
+Tensor int32(const Tensor& t) { return contig(t.scalar_type() == at::kInt ? t : t.to(at::kInt)); }
+}  // namespace
+
+std::vector<Tensor> expert_route(const Tensor& scores, const OptT& allowed_, int64_t k, bool normalize) {
+  const Tensor allowed = contig(opt(allowed_));
+  same_device("expert_route", scores, {&allowed});
+  if (any_grad({&scores})) return ExpertRoute::apply(scores, wrap(allowed), k, normalize);
+  return ExpertRoute::forward(nullptr, scores, wrap(allowed), k, normalize);
 }
 
 std::vector<Tensor> expert_plan(const Tensor& idx_, int64_t experts) {
@@ -219,25 +229,42 @@ std::vector<Tensor> expert_plan(const Tensor& idx_, int64_t experts) {
 }
 
 Tensor expert_dispatch(const Tensor& x, const Tensor& rows, const Tensor& offsets) {
+  same_device("expert_dispatch", x, {&rows, &offsets});
   if (any_grad({&x})) return ExpertDispatch::apply(x, rows, offsets);
   return ExpertDispatch::forward(nullptr, x, rows, offsets);
 }
 
-Tensor expert_combine(const Tensor& y, const Tensor& w, const Tensor& rows, const Tensor& offsets) {
+Tensor expert_combine(const Tensor& y, const Tensor& w_, const Tensor& rows, const Tensor& offsets) {
+  same_device("expert_combine", y, {&w_, &rows, &offsets});
+  const Tensor w = w_.scalar_type() == at::kFloat ? w_ : w_.to(at::kFloat);
   if (any_grad({&y, &w})) return ExpertCombine::apply(y, w, rows, offsets);
   return ExpertCombine::forward(nullptr, y, w, rows, offsets);
 }
 
-Tensor expert_linear(const Tensor& x, const Tensor& w, const Tensor& offsets, int64_t columns, bool accum) {
+Tensor expert_linear(const Tensor& x, const Tensor& w, const Tensor& offsets_, int64_t columns, bool accum) {
+  same_device("expert_linear", x, {&w, &offsets_});
+  const Tensor offsets = int32(offsets_);
   if (any_grad({&x, &w})) return ExpertLinear::apply(x, w, offsets, columns, accum);
   return ExpertLinear::forward(nullptr, x, w, offsets, columns, accum);
 }
 
-Tensor linear_4bit(const Tensor& x, const Tensor& codes, const Tensor& scale, const OptT& offsets, const OptT& bias_, int64_t experts,
-                   int64_t N, int64_t block, bool nf4) {
-  const Tensor bias = opt(bias_);
-  if (any_grad({&x, &bias})) return Linear4bit::apply(x, codes, scale, offsets, bias_, experts, N, block, nf4);
-  return Linear4bit::forward(nullptr, x, codes, scale, offsets, bias_, experts, N, block, nf4);
+// Nothing where the codes are not laid out for the kernel.
+OptT linear_4bit(const Tensor& x, const Tensor& codes, const Tensor& scale_, const OptT& offsets_, const OptT& bias_, int64_t experts,
+                 int64_t N, int64_t block, bool nf4) {
+  const Tensor bias = contig(opt(bias_));
+  Tensor offsets = opt(offsets_);
+  same_device("linear_4bit", x, {&codes, &scale_, &offsets, &bias});
+  if (!codes.is_contiguous() || !al16(codes)) return OptT();
+  if (offsets.defined()) offsets = int32(offsets);
+  const Tensor scale = contig(scale_.scalar_type() == at::kFloat ? scale_ : scale_.to(at::kFloat));
+  const int64_t K = x.size(-1);
+  const Tensor x2 = x.dim() == 2 ? x : x.reshape({-1, K});
+  Tensor y = any_grad({&x2, &bias}) ? Linear4bit::apply(x2, codes, scale, wrap(offsets), wrap(bias), experts, N, block, nf4)
+                                    : Linear4bit::forward(nullptr, x2, codes, scale, wrap(offsets), wrap(bias), experts, N, block, nf4);
+  if (x.dim() == 2) return y;
+  auto shape = x.sizes().vec();
+  shape.back() = N;
+  return y.view(shape);
 }
 
 }  // namespace eri_ops

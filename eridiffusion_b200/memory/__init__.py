@@ -219,7 +219,8 @@ def dequantize(q: QuantizedTensor, dtype=torch.bfloat16, out=None):
 
 class QuantizedLinear(nn.Module):
     """Frozen base weight stored quantised; dequantised per call into a scratch tensor and fed to
-    the fused linear (adapters attach as usual)."""
+    the fused linear (adapters attach as usual). A few rows on a 4-bit weight without adapter (conditioning
+    vectors) are multiplied with the codes themselves."""
 
     def __init__(self, linear, kind="int8", block=64):
         super().__init__()
@@ -240,6 +241,11 @@ class QuantizedLinear(nn.Module):
         from ..ops import functional as F
         if self.adapter is not None:
             return self.adapter(self, x, act=act, residual=residual, gate=gate)
+        if F.on_codes(x, self.q):
+            y = F.linear_4bit(x, self.q, bias=self.bias)
+            if act is not None:
+                y = F.gelu_tanh(y) if act == "gelu" else F.silu(y)
+            return y if gate is None and residual is None else F.gate_residual(residual, y, gate)
         return F.linear(x, self.weight, self.bias, act=act, residual=residual, gate=gate)
 
 

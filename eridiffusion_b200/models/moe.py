@@ -4,7 +4,9 @@ Reference: ``QuantKind{None, Q8, NF4}``, ``QWeight``, ``quantize_weight`` / ``de
 ``ExpertBank{insert, fetch_topk_bf16}`` and ``select_topk_global`` (crates/models/wan22/src/
 moe_quant.rs:6-48). In the reference the quantiser is a pass-through and the selection returns the
 first k ids. Here the bank stores real int8 / NF4 codes (``memory.quantize``; expanded by the
-dequantisation kernel on the GPU) and the selection is a top-k over router scores.
+dequantisation kernel on the GPU) and the selection is a top-k over router scores. On the GPU the tokens
+are put into expert order (``F.expert_plan`` / ``expert_dispatch``), meet all experts in one grouped product
+(``F.expert_linear``, or ``F.linear_4bit`` on the codes of a 4-bit bank) and are added up again (``F.expert_combine``).
 
 Wan 2.2 itself is not token-routed: its two "experts" are two whole transformers chosen by the
 timestep (``models/nextdit.py``: ``WanDualExpert``); the bank serves that case too (two entries,
@@ -17,6 +19,7 @@ import enum
 import torch
 
 from ..memory import QuantizedTensor, dequantize, quantize
+from ..ops import functional as F
 
 
 class QuantKind(str, enum.Enum):
@@ -40,6 +43,7 @@ class ExpertBank:
     def __init__(self, kind: QuantKind | str = QuantKind.Q8):
         self.kind = QuantKind(kind)
         self.experts: dict[int, object] = {}
+        self._stack = None              # (ids, their entries, stacked weight)
 
     def insert(self, expert_id: int, weight):
         """``weight``: a tensor (quantised on insertion) or an already quantised weight."""
@@ -57,6 +61,35 @@ class ExpertBank:
         return [(int(i), dequantize_to_bf16(self.experts[int(i)])) for i in ids if int(i) in self.experts]
 
 
+    def stacked(self, ids):
+        """The weights of the present experts ``ids`` as one [len(ids), N, K] tensor or, for 4-bit codes, one ``QuantizedTensor`` of
+        that shape. The bank's entries become views of it, so that nothing is held twice; it is made again when an entry
+        is replaced. None where they are of different shapes, kinds or devices, or stored as int8."""
+        ids = tuple(ids)
+        entries = [self.experts[i] for i in ids]
+        if self._stack is not None and self._stack[0] == ids and all(a is b for a, b in zip(self._stack[1], entries)):
+            return self._stack[2]
+        self._stack = None
+        first = entries[0]
+        if isinstance(first, QuantizedTensor):
+            key = [(e.kind, tuple(e.shape), e.block, e.data.device) if isinstance(e, QuantizedTensor) else None for e in entries]
+            if first.kind not in ("int4", "nf4") or len(first.shape) != 2 or any(k != key[0] for k in key):
+                return None
+            data, scale = torch.cat([e.data for e in entries]), torch.cat([e.scale for e in entries])
+            weight = QuantizedTensor(first.kind, data, scale, (len(ids), *first.shape), first.block)
+            per = first.data.shape[0]
+            views = [QuantizedTensor(first.kind, data[i * per:(i + 1) * per], scale[i * per:(i + 1) * per], first.shape, first.block)
+                     for i in range(len(ids))]
+        else:
+            if any(isinstance(e, QuantizedTensor) or e.dim() != 2 or e.shape != first.shape or e.device != first.device for e in entries):
+                return None
+            weight = torch.stack([e.to(torch.bfloat16) for e in entries])
+            views = list(weight.unbind(0))
+        self.experts.update(zip(ids, views))
+        self._stack = (ids, views, weight)
+        return weight
+
+
 def select_topk_global(scores_or_total, k: int):
     """With an int: the first ``k`` ids (the reference's behaviour). With router scores
     ``[tokens, experts]``: the ``k`` experts with the largest total probability mass over all
@@ -70,6 +103,13 @@ def select_topk_global(scores_or_total, k: int):
 def route_tokens(scores: torch.Tensor, k: int, allowed=None):
     """Per-token top-k routing: returns (expert ids [tokens, k], normalised weights [tokens, k]).
     ``allowed``: restrict the choice to these expert ids (the resident set)."""
+    if scores.is_cuda and scores.dim() == 2 and F.get_backend() == "fused":
+        mask = None
+        if allowed is not None:
+            mask = torch.zeros(scores.shape[1], dtype=torch.bool)
+            mask[list(allowed)] = True
+            mask = mask.to(scores.device)
+        return F.expert_route(scores, k, allowed=mask)
     s = scores.float()
     if allowed is not None:
         mask = torch.full_like(s, float("-inf"))
@@ -84,6 +124,9 @@ def moe_linear(x: torch.Tensor, scores: torch.Tensor, bank: ExpertBank, k: int =
     the experts some token uses (at most ``resident`` of them, chosen by ``select_topk_global``)."""
     allowed = select_topk_global(scores, resident) if resident else None
     idx, w = route_tokens(scores, k, allowed)
+    y = _moe_grouped(x, idx, w, scores.shape[-1], bank, allowed)
+    if y is not None:
+        return y
     out = None
     for e, We in bank.fetch_topk_bf16(sorted(set(idx.flatten().tolist()))):
         hit = idx == e                                              # [T, k]
@@ -93,3 +136,35 @@ def moe_linear(x: torch.Tensor, scores: torch.Tensor, bank: ExpertBank, k: int =
             out = torch.zeros(x.shape[0], We.shape[0], dtype=torch.float32, device=x.device)
         out[rows] += y.float() * (w * hit)[rows].sum(-1, keepdim=True)
     return out.to(x.dtype)
+
+
+def _moe_grouped(x, idx, w, total: int, bank: ExpertBank, allowed):
+    """``moe_linear`` as one grouped product on the GPU; None where that does not apply."""
+    if not (x.is_cuda and x.dtype == torch.bfloat16 and x.dim() == 2 and x.shape[0] > 0 and F.get_backend() == "fused"):
+        return None
+    ids = [i for i in (range(total) if allowed is None else sorted(allowed)) if i in bank.experts]
+    if not ids:
+        return None
+    weight = bank.stacked(ids)
+    if weight is None:
+        # int8 codes are expanded per expert: only those that some token uses
+        used = set(idx.flatten().tolist())
+        ids = [i for i in ids if i in used]
+        expanded = [dequantize_to_bf16(bank.experts[i]) for i in ids]
+        if not ids or any(e.dim() != 2 or e.shape != expanded[0].shape for e in expanded):
+            return None
+        weight = torch.stack(expanded)
+    stack_device = weight.data.device if isinstance(weight, QuantizedTensor) else weight.device
+    if stack_device != x.device or weight.shape[-1] != x.shape[1]:
+        return None
+    if len(ids) != total:                # the experts' places in the stack; an absent expert adds nothing
+        place = torch.full((total,), -1, dtype=torch.int64)
+        place[ids] = torch.arange(len(ids))
+        idx = place.to(x.device)[idx]
+    plan = F.expert_plan(idx, len(ids))
+    rows = F.expert_dispatch(x, plan)
+    if isinstance(weight, QuantizedTensor):
+        y = F.linear_4bit(rows, weight, plan.offsets)
+    else:
+        y = F.expert_linear(rows, weight, plan.offsets)
+    return F.expert_combine(y, w, plan)

@@ -965,10 +965,7 @@ def _same_device(what, *ts):
         raise ValueError(f"{what}: tensors on different devices: {sorted(str(d) for d in devices)}")
 
 
-def _experts_native(*ts) -> bool:
-    return _BACKEND == "fused" and all(t.is_cuda for t in ts) and N.require() is not None
-
-
+# The native nodes check devices and offsets themselves (a ValueError, too): the calls of a few rows are bound by the host.
 def expert_route(scores, k, allowed=None, normalize=True):
     """Router of a token: ``scores`` [T, E] -> (expert ids [T, k] int64, weights [T, k] fp32), the ``k`` largest scores in descending
     order, equal ones by lower index. ``normalize``: the weights are the softmax over the chosen scores (they add up to 1), else
@@ -982,10 +979,10 @@ def expert_route(scores, k, allowed=None, normalize=True):
     if allowed is not None:
         if allowed.dtype != torch.bool or allowed.shape != (E,):
             raise ValueError(f"expert_route: allowed must be a boolean [{E}], got {tuple(allowed.shape)} {allowed.dtype}")
-        _same_device("expert_route", scores, allowed)
-    if _experts_native(scores) and scores.dtype in (torch.float32, torch.bfloat16) and T > 0 and E <= _MAX_EXPERTS and k <= _MAX_TOP:
-        idx, w = N.ops().expert_route(scores, _c(allowed), k, bool(normalize))
-        return idx, w
+    if scores.is_cuda and _BACKEND == "fused" and scores.dtype in (torch.float32, torch.bfloat16) and T > 0 and E <= _MAX_EXPERTS \
+            and k <= _MAX_TOP:
+        return tuple(N.ops().expert_route(scores, allowed, k, normalize))
+    _same_device("expert_route", scores, allowed)
     return R.expert_route(scores, k, allowed, normalize)
 
 
@@ -995,7 +992,7 @@ def expert_plan(idx, num_experts) -> ExpertPlan:
         raise ValueError(f"expert_plan: idx must be [tokens, k] int64 or int32, got {tuple(idx.shape)} {idx.dtype}")
     if num_experts < 1 or idx.numel() >= 2 ** 31:
         raise ValueError(f"expert_plan: {num_experts} experts, {idx.numel()} choices")
-    if _experts_native(idx) and num_experts <= _MAX_EXPERTS:
+    if idx.is_cuda and _BACKEND == "fused" and num_experts <= _MAX_EXPERTS:
         return ExpertPlan(*N.ops().expert_plan(idx, num_experts))
     return ExpertPlan(*R.expert_plan(idx, num_experts))
 
@@ -1005,9 +1002,9 @@ def expert_dispatch(x, plan: ExpertPlan):
     T, k = plan.rows.shape
     if x.dim() != 2 or x.shape[0] != T:
         raise ValueError(f"expert_dispatch: x {tuple(x.shape)} for a plan of {T} tokens")
-    _same_device("expert_dispatch", x, plan.rows)
     if _native_ok(x) and x.shape[1] % 8 == 0 and x.numel() > 0:
         return N.ops().expert_dispatch(x, plan.rows, plan.offsets)
+    _same_device("expert_dispatch", x, plan.rows)
     return R.expert_dispatch(x, plan.source, k)
 
 
@@ -1016,16 +1013,15 @@ def expert_combine(y, weights, plan: ExpertPlan):
     T, k = plan.rows.shape
     if y.dim() != 2 or y.shape[0] != T * k or tuple(weights.shape) != (T, k):
         raise ValueError(f"expert_combine: y {tuple(y.shape)}, weights {tuple(weights.shape)} for a plan of {T} tokens and {k} choices")
-    _same_device("expert_combine", y, weights, plan.rows)
     if _native_ok(y) and y.shape[1] % 8 == 0 and y.numel() > 0:
-        return N.ops().expert_combine(y, weights.float(), plan.rows, plan.offsets)
+        return N.ops().expert_combine(y, weights, plan.rows, plan.offsets)
+    _same_device("expert_combine", y, weights, plan.rows)
     return R.expert_combine(y, weights, plan.rows)
 
 
-def _check_offsets(what, offsets, E, x):
+def _check_offsets(what, offsets, E):
     if offsets.dim() != 1 or offsets.shape[0] != E + 1 or offsets.dtype not in (torch.int32, torch.int64):
         raise ValueError(f"{what}: offsets must be [{E + 1}] int32 or int64, got {tuple(offsets.shape)} {offsets.dtype}")
-    _same_device(what, x, offsets)
 
 
 def expert_linear(x, w, offsets):
@@ -1034,18 +1030,25 @@ def expert_linear(x, w, offsets):
     Differentiable in x and w; nothing is read back to the host."""
     if x.dim() != 2 or w.dim() != 3 or x.shape[1] != w.shape[2] or w.shape[0] < 1:
         raise ValueError(f"expert_linear: x {tuple(x.shape)} and w {tuple(w.shape)} must be [R, K] and [E, N, K]")
-    _check_offsets("expert_linear", offsets, w.shape[0], x)
-    _same_device("expert_linear", x, w)
+    E, Nn, K = w.shape
+    _check_offsets("expert_linear", offsets, E)
     if x.dtype != w.dtype:
         raise ValueError(f"expert_linear: x {x.dtype}, w {w.dtype}")
-    E, Nn, K = w.shape
     if _native_ok(x, w) and E <= _MAX_EXPERTS and Nn % 8 == 0 and K % 8 == 0 and Nn > 0 and K > 0 and x.shape[0] < 2 ** 31:
-        return N.ops().expert_linear(x, w, offsets.to(torch.int32).contiguous(), 0, _ACCUM_INTO_GRAD)
+        return N.ops().expert_linear(x, w, offsets, 0, _ACCUM_INTO_GRAD)
+    _same_device("expert_linear", x, w, offsets)
     return R.expert_linear(x, w, offsets)
 
 
-# Most rows that are multiplied with the codes themselves; above, the weight is expanded once and meets the matrix kernels.
-_CODES_ROWS, _CODES_EXPERT_ROWS = 8, 64
+# Most rows that are multiplied with the codes themselves; above, the weight is expanded once and meets the matrix kernels. Widest row:
+# x of a pass, the rings and the tables share an SM's memory.
+_CODES_ROWS, _CODES_EXPERT_ROWS, _CODES_WIDTH = 8, 64, 16384
+
+
+def on_codes(x, q) -> bool:
+    """Whether ``linear_4bit`` multiplies x with the codes of the dense weight ``q`` themselves."""
+    return (q.kind in ("int4", "nf4") and len(q.shape) == 2 and _native_ok(x) and x.numel() <= _CODES_ROWS * q.shape[1]
+            and q.shape[1] <= _CODES_WIDTH and q.shape[1] % q.block == 0 and q.block % 32 == 0)
 
 
 def linear_4bit(x, q, offsets=None, bias=None):
@@ -1053,28 +1056,33 @@ def linear_4bit(x, q, offsets=None, bias=None):
     [..., K]. ``q.shape`` [E, N, K] with ``offsets`` [E + 1]: x [R, K] in expert order, as in ``expert_linear``. A few bf16 rows
     on the GPU are multiplied with the codes (the weight in full precision ``level * scale``); more rows expand the weight to bf16
     first. Differentiable in x and bias."""
-    if q.kind not in ("int4", "nf4"):
+    nf4 = q.kind == "nf4"
+    if not nf4 and q.kind != "int4":
         raise ValueError(f"linear_4bit: {q.kind} weights")
-    experts = len(q.shape) == 3
-    if len(q.shape) not in (2, 3) or experts != (offsets is not None):
-        raise ValueError(f"linear_4bit: a weight of shape {tuple(q.shape)} {'needs' if experts else 'takes no'} offsets")
-    E, (Nn, K) = (q.shape[0] if experts else 1), q.shape[-2:]
-    if x.shape[-1:] != (K,) or (experts and x.dim() != 2):
-        raise ValueError(f"linear_4bit: x {tuple(x.shape)} for a weight of shape {tuple(q.shape)}")
+    shape = q.shape
+    Nn, K = shape[-2:]
+    experts = len(shape) == 3
     if experts:
-        _check_offsets("linear_4bit", offsets, E, x)
-        if bias is not None:
-            raise ValueError("linear_4bit: no bias with offsets")
-    elif bias is not None and tuple(bias.shape) != (Nn,):
-        raise ValueError(f"linear_4bit: bias {tuple(bias.shape)} for {Nn} outputs")
-    _same_device("linear_4bit", x, q.data, q.scale, bias)
-    rows = x.numel() // K
-    if _native_ok(x, bias) and rows <= (_CODES_EXPERT_ROWS if experts else _CODES_ROWS) and E <= _MAX_EXPERTS and K % q.block == 0 and q.block % 32 == 0 \
-            and q.data.is_contiguous() and q.data.data_ptr() % 16 == 0 and Nn > 0:
-        y = N.ops().linear_4bit(x.reshape(rows, K), q.data, q.scale.float().contiguous(),
-                                None if offsets is None else offsets.to(torch.int32).contiguous(), bias, E, Nn, q.block, q.kind == "nf4")
-        return y.view(*x.shape[:-1], Nn)
-    if _native_ok(x):
+        E = shape[0]
+        if offsets is None or bias is not None or x.dim() != 2:
+            raise ValueError(f"linear_4bit: a weight of shape {tuple(shape)} takes rows [R, {K}], offsets and no bias")
+        _check_offsets("linear_4bit", offsets, E)
+    else:
+        E = 1
+        if len(shape) != 2 or offsets is not None:
+            raise ValueError(f"linear_4bit: a weight of shape {tuple(shape)} takes no offsets")
+        if bias is not None and tuple(bias.shape) != (Nn,):
+            raise ValueError(f"linear_4bit: bias {tuple(bias.shape)} for {Nn} outputs")
+    if x.shape[-1:] != (K,):
+        raise ValueError(f"linear_4bit: x {tuple(x.shape)} for a weight of shape {tuple(shape)}")
+    native = _native_ok(x, bias)
+    if native and x.numel() <= (_CODES_EXPERT_ROWS if experts else _CODES_ROWS) * K and E <= _MAX_EXPERTS and K <= _CODES_WIDTH \
+            and K % q.block == 0 and q.block % 32 == 0 and Nn > 0:
+        y = N.ops().linear_4bit(x, q.data, q.scale, offsets, bias, E, Nn, q.block, nf4)
+        if y is not None:
+            return y
+    _same_device("linear_4bit", x, q.data, q.scale, bias, offsets)
+    if native:
         w = q.dequantize(torch.bfloat16)
         return expert_linear(x, w, offsets) if experts else linear(x, w, bias)
     return R.linear_4bit(x, q.dequantize(torch.float32), offsets, bias)
