@@ -365,9 +365,9 @@ expert_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constan
     for (int t = first; t < sched.total; t += stride, ++it) {
       const Tile tl = sched.get(t);
       const int buf = it & 1;
-      if (!mbar_wait(&acc_full[buf], (uint32_t)(it >> 1) & 1)) {
+      if (!failed && !mbar_wait(&acc_full[buf], (uint32_t)(it >> 1) & 1)) {
         if (lane == 0) atomicExch(&g_err, 44);
-        failed = true;
+        failed = true;                               // no further wait; what is left becomes NaN
       }
       tc_fence_after();
       const int p0 = tl.p0 + (int)rank * BM;
@@ -376,7 +376,7 @@ expert_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constan
       const int col0 = half * C::kHalf;
       const int cols = MODE == kDw ? min(C::kHalf, p.C - tl.c0 - col0) : min(C::kHalf, tl.hi - tl.lo - col0);
       bf16* o = p.out + (MODE == kDw ? ((long long)tl.e * p.C + tl.c0 + col0) : (long long)(tl.lo + col0)) * p.P + p0 + v_col;
-      const bool v_ok = p0 + v_col < p.P && !failed;
+      const bool v_ok = p0 + v_col < p.P;
       uint32_t r[2][8];                              // the two halves of the quadrant
       if (cols > 0) {
         tmem_ld_16x16(acc, r[0]);
@@ -398,7 +398,7 @@ expert_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constan
         for (int h = 0; h < 2; ++h) {
           float f[8];
 #pragma unroll
-          for (int i = 0; i < 8; ++i) f[i] = MODE == kDw && tl.steps == 0 ? 0.f : __uint_as_float(r[h][i]);     // (an expert without rows)
+          for (int i = 0; i < 8; ++i) f[i] = failed ? __int_as_float(0x7fffffff) : MODE == kDw && tl.steps == 0 ? 0.f : __uint_as_float(r[h][i]);     // (an expert without rows)
           if (MODE == kDw && p.accum) {
             uint32_t old[4];
             load_blocks_t(s_m + h * 32, old);

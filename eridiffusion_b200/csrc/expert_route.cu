@@ -166,14 +166,13 @@ __global__ void __launch_bounds__(256) route_bwd_kernel(const T* __restrict__ sc
 #pragma unroll
     for (int i = 0; i < VPL; ++i) {
       const float p = m == kNegInf ? 0.f : __fdiv_rn(exp_nonpos(v[i] - m), sum);
-      const bool open = lane + 32 * i < E && (!allowed || allowed[lane + 32 * i]);
-      g[i] = open ? p * (g[i] - dot) : 0.f;
+      g[i] = p * (g[i] - dot);
     }
   }
   T* out = ds + (long long)t * E;
 #pragma unroll
   for (int i = 0; i < VPL; ++i)
-    if (lane + 32 * i < E) store_score(out + lane + 32 * i, g[i]);
+    if (lane + 32 * i < E) store_score(out + lane + 32 * i, !allowed || allowed[lane + 32 * i] ? g[i] : 0.f);
 }
 
 // ------------------------------------------------------------------------------------------- plan

@@ -134,9 +134,10 @@ struct PieceRing {
   }
   // place of a row's 16-byte chunk (rows 32 / kChunks apart are permuted alike)
   static __device__ __forceinline__ int chunk(int row, int c) { return STEP == 64 ? c ^ ((row << 1) & 7) : c ^ ((row >> 1) & 3); }
-  // pieces lo .. hi - 1 of the 16-row tiles first, first + step, ... below end; everything fetched before has been read
+  // pieces lo .. hi - 1 of the 16-row tiles first, first + step, ... below end; everything fetched before has been read by every lane
   __device__ __forceinline__ void start(const Weight& w, int e, int lane, int first, int end, int step, int lo, int hi) {
     tile = first; tile_end = end; tile_step = step; p_lo = piece = lo; p_hi = hi;
+    put = get = 0;
     const long long row = (long long)e * w.N + 16ll * first;
     tile_bytes = 16ll * step * w.k_bytes - (long long)(hi - lo) * kRow;
     tile_scales = 16ll * step * w.spr;

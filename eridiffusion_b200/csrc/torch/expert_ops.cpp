@@ -207,6 +207,10 @@ void same_device(const char* what, const Tensor& a, std::initializer_list<const 
   for (const Tensor* t : ts)
     TORCH_CHECK_VALUE(!t->defined() || t->device() == a.device(), what, ": tensors on different devices: ", a.device(), " and ", t->device());
 }
+void check_plan(const char* what, const Tensor& rows, const Tensor& offsets) {
+  TORCH_CHECK_VALUE(rows.scalar_type() == at::kInt && rows.is_contiguous() && offsets.scalar_type() == at::kInt && offsets.is_contiguous() &&
+                        offsets.dim() == 1 && offsets.size(0) > 1, what, ": not a plan of expert_plan");
+}
 Tensor int32(const Tensor& t) { return contig(t.scalar_type() == at::kInt ? t : t.to(at::kInt)); }
 }  // namespace
 
@@ -230,12 +234,14 @@ std::vector<Tensor> expert_plan(const Tensor& idx_, int64_t experts) {
 
 Tensor expert_dispatch(const Tensor& x, const Tensor& rows, const Tensor& offsets) {
   same_device("expert_dispatch", x, {&rows, &offsets});
+  check_plan("expert_dispatch", rows, offsets);
   if (any_grad({&x})) return ExpertDispatch::apply(x, rows, offsets);
   return ExpertDispatch::forward(nullptr, x, rows, offsets);
 }
 
 Tensor expert_combine(const Tensor& y, const Tensor& w_, const Tensor& rows, const Tensor& offsets) {
   same_device("expert_combine", y, {&w_, &rows, &offsets});
+  check_plan("expert_combine", rows, offsets);
   const Tensor w = w_.scalar_type() == at::kFloat ? w_ : w_.to(at::kFloat);
   if (any_grad({&y, &w})) return ExpertCombine::apply(y, w, rows, offsets);
   return ExpertCombine::forward(nullptr, y, w, rows, offsets);

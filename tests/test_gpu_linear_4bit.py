@@ -26,9 +26,10 @@ def _weight64(q):
     return (v * q.scale.double()[:, None]).view(q.shape)
 
 
-def _near(a, ref, mag, terms):
-    # sums, a level's 2^-11 and the scale of a row's block as a power of two; the rounding to bf16
-    bad = ~((a.double() - ref).abs() <= ref.abs() * 2 ** -8 + mag * (terms * 2 ** -23 + 2 ** -11))
+def _near(a, ref, mag, terms, expanded=False):
+    # sums, a level's 2^-11 and the scale of a row's block as a power of two; the rounding to bf16. More rows than are multiplied with
+    # the codes meet the weight expanded to bf16: every weight, and with it every product, is off by up to 2^-8 of itself
+    bad = ~((a.double() - ref).abs() <= ref.abs() * 2 ** -8 + mag * (terms * 2 ** -23 + (2 ** -8 if expanded else 2 ** -11)))
     assert a.shape == ref.shape and not bad.any(), (int(bad.sum()), bad.nonzero()[:4].tolist(), a[bad][:4].tolist(), ref[bad][:4].tolist())
 
 
@@ -156,3 +157,34 @@ def test_in_a_graph():
         graph.replay()
         fresh = F.linear_4bit(x, q, off)
         assert torch.equal(y, fresh) and torch.equal(dx, torch.autograd.grad(fresh, x, dy)[0])
+
+
+@pytest.mark.parametrize("kind", ["int4", "nf4"])
+@pytest.mark.parametrize("E,N,K,block", [(64, 2000, 320, 64), (48, 2000, 320, 64), (40, 1208, 1024, 64), (24, 3000, 160, 32)])
+def test_many_experts_per_cta(E, N, K, block, kind):
+    """More tiles than CTAs, so that a CTA goes on from one expert's rows to the next one's."""
+    g = _gen(E + N)
+    q = _random(g, kind, (E, N, K), block)
+    counts = [1 + (i % 3 == 0) - (i % 7 == 3) for i in range(E)]
+    off = torch.tensor([0, *counts]).cumsum(0).to(torch.int32).cuda()
+    R = sum(counts)
+    x, dy = _mk(g, R, K).requires_grad_(), _mk(g, R, N)
+    y = F.linear_4bit(x, q, off)
+    (dx,) = torch.autograd.grad(y, x, dy)
+    we = _weight64(q)[torch.repeat_interleave(torch.arange(E), torch.tensor(counts)).cuda()]
+    xd, dd, expanded = x.detach().double(), dy.double(), R > F._CODES_EXPERT_ROWS       # (the first case: 77 rows)
+    _near(y.detach(), torch.einsum("rk,rnk->rn", xd, we), torch.einsum("rk,rnk->rn", xd.abs(), we.abs()), K, expanded)
+    _near(dx, torch.einsum("rn,rnk->rk", dd, we), torch.einsum("rn,rnk->rk", dd.abs(), we.abs()), N, expanded)
+
+
+@pytest.mark.parametrize("kind", ["int4", "nf4"])
+def test_long_rows_take_several_passes(kind):
+    """x of eight rows does not fit next to the rings: the codes are read once per few rows."""
+    g = _gen(17)
+    q = _random(g, kind, (50, 16384), 64)
+    x, dy = _mk(g, 8, 16384).requires_grad_(), _mk(g, 8, 50)
+    y = F.linear_4bit(x, q)
+    (dx,) = torch.autograd.grad(y, x, dy)
+    w = _weight64(q)
+    _near(y.detach(), x.detach().double() @ w.t(), x.detach().double().abs() @ w.abs().t(), 16384)
+    _near(dx, dy.double() @ w, dy.double().abs() @ w.abs(), 50)
