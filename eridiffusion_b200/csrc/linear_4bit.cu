@@ -645,8 +645,15 @@ int launch4d(const Args4& p, int grid, int smem, int dev, cudaStream_t st) {
 
 template <bool NF4, int STEP>
 int launch4(Args4& p, int dev, cudaStream_t st) {
-  const int steps = p.K / STEP, pieces = (steps + kU - 1) / kU, turns = (pieces + kMaxSplit - 1) / kMaxSplit, tiles = (p.N + 15) / 16;
-  const int piece = 16 * kU * STEP / 2 + 16 * kU * 4, want = min_of(kRows, p.R);
+  const int steps = p.K / STEP, pieces = (steps + kU - 1) / kU, tiles = (p.N + 15) / 16;
+  const int piece = 16 * kU * STEP / 2 + 16 * kU * 4, want = min_of(kRows, p.R), sms = num_sms(dev);
+  // Ten warps share a tile where there are few tiles, five where every warp gets some pieces all the same: their barrier and final sum come
+  // half as often. us, K = 2560, one NF4 row, ten | five: 16 x K 4.6 | 4.8, 15360 x K 12.2 | 12.7, 18944 x K 13.6 | 13.0,
+  // 75776 x K 41.3 | 36.8; K = 5120, eight int4 rows: 16 x K 7.8 | 10.4, 15360 x K 21.5 | 19.9. (About every second row of the
+  // grouped form starts a pass.)
+  const long long most_pieces = (long long)tiles * pieces * (p.offsets ? (p.R + 1) / 2 : 1);
+  const int split = most_pieces >= 4ll * kMaxWarps * sms ? kMaxSplit / 2 : kMaxSplit;
+  const int turns = (pieces + split - 1) / split;
   p.kw = (pieces + turns - 1) / turns;
   // Two CTAs of half the warps share an SM where all rows of x fit: one's prologue and last tiles run beside the other. Shared memory: the
   // table, every warp's ring of three pieces (two, where that makes room for x), partial sums, x of a pass; fewer rows per pass
@@ -666,7 +673,7 @@ int launch4(Args4& p, int dev, cudaStream_t st) {
   // in the grouped form each row may be a pass of its own
   const long long most = (long long)(p.offsets ? p.R : (p.R + p.rows - 1) / p.rows) * ((tiles + p.nw - 1) / p.nw);
   if (most > 0x7fffffff) return -100;
-  const int ctas = per_sm * num_sms(dev), grid = most < ctas ? (int)most : ctas;
+  const int ctas = per_sm * sms, grid = most < ctas ? (int)most : ctas;
   if (depth == 3) return steps % kU ? launch4d<NF4, STEP, false, 3>(p, grid, smem, dev, st) : launch4d<NF4, STEP, true, 3>(p, grid, smem, dev, st);
   return steps % kU ? launch4d<NF4, STEP, false, 2>(p, grid, smem, dev, st) : launch4d<NF4, STEP, true, 2>(p, grid, smem, dev, st);
 }
