@@ -1,7 +1,7 @@
 // Token-routed experts: the router, the order of the routed rows, and the copies into and out of that order.
 //
 //   eri_expert_route_fwd / _bwd   the k largest scores of a row (ties: the lower index) with softmax weights, and the gradient
-//   eri_expert_plan               stable counting sort of the chosen experts: offsets, row of every choice, choice of every row
+//   eri_expert_plan               stable counting sort of the chosen experts: offsets and the row of every choice
 //   eri_expert_scatter            xs[rows[t, j]] = x[t]                      (into expert order)
 //   eri_expert_gather             out[t] = sum_j w[t, j] y[rows[t, j]]       (back; w == nullptr: all ones, the scatter's gradient)
 //   eri_expert_gather_bwd         dy[rows[t, j]] = w[t, j] dout[t], dw[t, j] = <dout[t], y[rows[t, j]]>
@@ -212,14 +212,12 @@ __device__ __forceinline__ int ld_cluster(uint32_t addr) {      // not ordered a
 }
 
 __global__ void __launch_bounds__(kPlanThreads) expert_plan_kernel(const void* __restrict__ idx, int wide, int n, int E, int ctas,
-                                                                   int* __restrict__ offsets, int* __restrict__ rows,
-                                                                   int* __restrict__ source) {
+                                                                   int* __restrict__ offsets, int* __restrict__ rows) {
   extern __shared__ int plan_smem[];
   int* total = plan_smem;                 // [E] this CTA's choices of every expert
   int* base = total + E;                  // [E] rows of lower CTAs of the expert
   int* first = base + E;                  // [E] first row of the expert
   int* cnt = first + E;                   // [kPlanWarps][E]
-  __shared__ int s_live;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int rank = ctas > 1 ? (int)cluster_ctarank() : 0;
   const int warps = ctas * kPlanWarps;
@@ -292,10 +290,7 @@ __global__ void __launch_bounds__(kPlanThreads) expert_plan_kernel(const void* _
       }
       run += __shfl_sync(0xffffffffu, scan, 31);
     }
-    if (lane == 0) {
-      s_live = run;
-      if (rank == 0) offsets[E] = run;
-    }
+    if (lane == 0 && rank == 0) offsets[E] = run;
   }
   __syncthreads();
   const bool held = piece <= 32 * kHold;
@@ -312,13 +307,11 @@ __global__ void __launch_bounds__(kPlanThreads) expert_plan_kernel(const void* _
         if (c[u] >= 0 && lane == __ffs(same[u]) - 1) mine[c[u]] += __popc(same[u]);
         __syncwarp();
         if (i < hi) {
-          rows[i] = pos;
-          if (pos >= 0 && ERI_DBG_INDEX(pos, n, 71)) source[pos] = (int)i;
+          if (pos < 0 || ERI_DBG_INDEX(pos, n, 71)) rows[i] = pos;
         }
       }
     }
   }
-  for (long long i = (long long)s_live + rank * kPlanThreads + threadIdx.x; i < n; i += (long long)ctas * kPlanThreads) source[i] = -1;
   if (ctas > 1) asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
 
@@ -532,8 +525,8 @@ int eri_expert_route_bwd(const void* scores, long long ld, const void* allowed, 
                  : route_bwd<float>(scores, ld, allowed, (const long long*)idx, w, dw, ds, tokens, E, k, normalize, st);
 }
 
-// idx: n choices (int64 when wide, else int32). offsets [E + 1], rows [n], source [n] int32.
-int eri_expert_plan(const void* idx, int wide, int n, int E, int* offsets, int* rows, int* source, void* stream) {
+// idx: n choices (int64 when wide, else int32). offsets [E + 1], rows [n] int32.
+int eri_expert_plan(const void* idx, int wide, int n, int E, int* offsets, int* rows, void* stream) {
   if (n < 0 || E < 1 || E > kMaxExperts) return -1;
   const int smem = (kPlanWarps + 3) * E * (int)sizeof(int);
   int dev = 0;
@@ -556,7 +549,7 @@ int eri_expert_plan(const void* idx, int wide, int n, int E, int* offsets, int* 
   at[0].val.clusterDim.x = ctas; at[0].val.clusterDim.y = 1; at[0].val.clusterDim.z = 1;
   cfg.attrs = at;
   cfg.numAttrs = ctas > 1 ? 1 : 0;
-  return (int)cudaLaunchKernelEx(&cfg, expert_plan_kernel, idx, wide, n, E, ctas, offsets, rows, source);
+  return (int)cudaLaunchKernelEx(&cfg, expert_plan_kernel, idx, wide, n, E, ctas, offsets, rows);
 }
 
 // x [tokens, D] (row stride ldx) -> xs [n_rows, D]; live: offsets + E.

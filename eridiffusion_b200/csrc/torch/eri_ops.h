@@ -85,7 +85,7 @@ using torch::autograd::variable_list;
   X(eri_expert_route_fwd, (const void*, long long, const void*, void*, float*, int, int, int, int, int, void*))  \
   X(eri_expert_route_bwd, (const void*, long long, const void*, const void*, const float*, const float*, void*,  \
                            int, int, int, int, int, void*))                                                      \
-  X(eri_expert_plan, (const void*, int, int, int, int*, int*, int*, void*))                                      \
+  X(eri_expert_plan, (const void*, int, int, int, int*, int*, void*))                                            \
   X(eri_expert_scatter, (const void*, long long, const int*, const int*, void*, int, int, int, int, void*))      \
   X(eri_expert_gather, (const void*, long long, const int*, const float*, void*, int, int, int, int, void*))     \
   X(eri_expert_gather_bwd, (const void*, long long, const void*, long long, const int*, const float*, const int*, \

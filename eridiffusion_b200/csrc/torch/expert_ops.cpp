@@ -226,10 +226,10 @@ std::vector<Tensor> expert_plan(const Tensor& idx_, int64_t experts) {
   const Tensor idx = contig(idx_);
   const auto o = idx.options().dtype(at::kInt);
   const int64_t n = idx.numel();
-  Tensor offsets = at::empty({experts + 1}, o), rows = at::empty(idx.sizes(), o), source = at::empty({n}, o);
+  Tensor offsets = at::empty({experts + 1}, o), rows = at::empty(idx.sizes(), o);
   check(L.eri_expert_plan(idx.data_ptr(), idx.scalar_type() == at::kLong, (int)n, (int)experts, (int*)offsets.data_ptr(),
-                          (int*)rows.data_ptr(), (int*)source.data_ptr(), stream()), "expert_plan");
-  return {offsets, rows, source};
+                          (int*)rows.data_ptr(), stream()), "expert_plan");
+  return {offsets, rows};
 }
 
 Tensor expert_dispatch(const Tensor& x, const Tensor& rows, const Tensor& offsets) {

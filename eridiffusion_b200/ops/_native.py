@@ -125,7 +125,7 @@ _SIGNATURES = {
     "eri_rows_dgrad": [_P, _I, _P, _I, _P, _I, _I, _I, _I, _P],
     "eri_expert_route_fwd": [_P, _L, _P, _P, _P, _I, _I, _I, _I, _I, _P],
     "eri_expert_route_bwd": [_P, _L, _P, _P, _P, _P, _P, _I, _I, _I, _I, _I, _P],
-    "eri_expert_plan": [_P, _I, _I, _I, _P, _P, _P, _P],
+    "eri_expert_plan": [_P, _I, _I, _I, _P, _P, _P],
     "eri_expert_scatter": [_P, _L, _P, _P, _P, _I, _I, _I, _I, _P],
     "eri_expert_gather": [_P, _L, _P, _P, _P, _I, _I, _I, _I, _P],
     "eri_expert_gather_bwd": [_P, _L, _P, _L, _P, _P, _P, _P, _P, _I, _I, _I, _I, _P],

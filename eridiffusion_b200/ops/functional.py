@@ -952,11 +952,9 @@ _MAX_EXPERTS, _MAX_TOP = 1024, 32         # what the router, the plan and the gr
 
 class ExpertPlan(NamedTuple):
     """Order of the routed rows: row r belongs to expert e for ``offsets[e] <= r < offsets[e + 1]`` (int32, on the device);
-    ``rows`` [T, k] is the row of every choice (-1: a choice outside [0, E), e.g. of a padding token), ``source`` [T * k] the
-    choice ``t * k + j`` of every row (-1 from ``offsets[E]`` on)."""
+    ``rows`` [T, k] is the row of every choice (-1: a choice outside [0, E), e.g. of a padding token)."""
     offsets: torch.Tensor
     rows: torch.Tensor
-    source: torch.Tensor
 
 
 def _same_device(what, *ts):
@@ -1005,7 +1003,7 @@ def expert_dispatch(x, plan: ExpertPlan):
     if _native_ok(x) and x.shape[1] % 8 == 0 and x.numel() > 0:
         return N.ops().expert_dispatch(x, plan.rows, plan.offsets)
     _same_device("expert_dispatch", x, plan.rows)
-    return R.expert_dispatch(x, plan.source, k)
+    return R.expert_dispatch(x, plan.rows)
 
 
 def expert_combine(y, weights, plan: ExpertPlan):

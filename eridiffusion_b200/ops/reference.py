@@ -237,7 +237,7 @@ def expert_route(scores, k, allowed=None, normalize=True):
 
 
 def expert_plan(idx, num_experts):
-    """(offsets [E + 1], rows [T, k], source [T * k]) int32 of the stable sort of the choices by expert."""
+    """(offsets [E + 1], rows [T, k]) int32 of the stable sort of the choices by expert."""
     flat = idx.reshape(-1).long()
     valid = (flat >= 0) & (flat < num_experts)
     key = torch.where(valid, flat, num_experts)
@@ -248,12 +248,15 @@ def expert_plan(idx, num_experts):
     rows = torch.empty_like(order)
     rows[order] = place
     rows = torch.where(valid, rows, -1).view(idx.shape)
-    return offsets.int(), rows.int(), torch.where(place < offsets[-1], order, -1).int()
+    return offsets.int(), rows.int()
 
 
-def expert_dispatch(x, source, k):
-    token = torch.div(source.clamp_min(0).long(), k, rounding_mode="floor")
-    return torch.where((source >= 0)[:, None], x.float()[token], 0.0).to(x.dtype)
+def expert_dispatch(x, rows):
+    T, k = rows.shape
+    here = rows.reshape(-1) >= 0
+    token = torch.arange(T, device=x.device).repeat_interleave(k)[here]
+    out = x.new_zeros(T * k, x.shape[1], dtype=torch.float32)
+    return out.index_copy(0, rows.reshape(-1)[here].long(), x.float()[token]).to(x.dtype)
 
 
 def expert_combine(y, w, rows):

@@ -105,9 +105,9 @@ def test_plan(T, k, E, dtype):
     g = _gen(T + k + E)
     idx = torch.randint(-1, E + (1 if T % 2 else 0), (T, k), device="cuda", generator=g).to(dtype)     # some outside [0, E)
     plan = F.expert_plan(idx, E)
-    offsets, rows, source = (t.cpu() for t in plan)
-    ro, rr, rs = F.R.expert_plan(idx.cpu(), E)
-    assert torch.equal(offsets, ro) and torch.equal(rows, rr) and torch.equal(source, rs)
+    offsets, rows = (t.cpu() for t in plan)
+    ro, rr = F.R.expert_plan(idx.cpu(), E)
+    assert torch.equal(offsets, ro) and torch.equal(rows, rr)
     again = F.expert_plan(idx, E)
     assert all(torch.equal(a, b) for a, b in zip(plan, again))
 
@@ -117,7 +117,7 @@ def test_plan_of_one_expert_only():
         plan = F.expert_plan(torch.full((n, 1), 3, device="cuda"), 5)
         assert plan.offsets.tolist() == [0, 0, 0, 0, n, n] and torch.equal(plan.rows[:, 0].cpu(), torch.arange(n, dtype=torch.int32))
         none = F.expert_plan(torch.full((n, 1), 9, device="cuda"), 5)
-        assert none.offsets.tolist() == [0] * 6 and (none.rows == -1).all() and (none.source == -1).all()
+        assert none.offsets.tolist() == [0] * 6 and (none.rows == -1).all()
 
 
 @pytest.mark.parametrize("T,k,E,D", [(1, 1, 1, 8), (7, 2, 32, 640), (65, 9, 12, 136), (300, 17, 40, 1288), (1000, 4, 8, 72)])
@@ -136,7 +136,10 @@ def test_dispatch_and_combine(T, k, E, D, padded):
     w = torch.rand(T, k, device="cuda", generator=g).requires_grad_()
     xs, out = F.expert_dispatch(x, plan), F.expert_combine(y, w, plan)
     rows, here = plan.rows.long().clamp_min(0), (plan.rows >= 0)
-    token = plan.source[:live].long() // k
+    flat = plan.rows.reshape(-1).long()
+    choice = torch.empty(live, dtype=torch.int64, device="cuda")          # of every row
+    choice[flat[flat >= 0]] = torch.arange(T * k, device="cuda")[flat >= 0]
+    token = choice // k
     assert torch.equal(xs[:live], x.detach()[token]) and (xs[live:] == 0).all()
     yt = torch.where(here[..., None], y.detach().double()[rows], 0.0)
     ref = (w.detach().double()[..., None] * yt).sum(1)
@@ -147,7 +150,7 @@ def test_dispatch_and_combine(T, k, E, D, padded):
     dx, dy, dw = torch.autograd.grad((xs, out), (x, y, w), (dxs, dout))
     dt = torch.where(here[..., None], dxs.double()[rows], 0.0)
     assert ((dx.double() - dt.sum(1)).abs() <= dt.sum(1).abs() * 2 ** -8 + dt.abs().sum(1) * k * 2 ** -23).all()
-    rdy = w.detach().double().reshape(-1)[plan.source[:live].long()][:, None] * dout.double()[token]
+    rdy = w.detach().double().reshape(-1)[choice][:, None] * dout.double()[token]
     assert ((dy[:live].double() - rdy).abs() <= rdy.abs() * (2 ** -8 + 2 ** -23)).all() and (dy[live:] == 0).all()
     prod = yt * dout.double()[:, None]
     assert ((dw.double() - prod.sum(-1)).abs() <= prod.abs().sum(-1) * D * 2 ** -23).all() and (dw[~here] == 0).all()

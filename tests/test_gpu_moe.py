@@ -87,8 +87,8 @@ def _feed_forward(x, scores, w1, w2, k):
 def _feed_forward_ref(x, scores, w1, w2, k):
     """The same with PyTorch statements on the given types."""
     idx, w = F.R.expert_route(scores, k)
-    off, rows, src = F.R.expert_plan(idx, w1.shape[0])
-    h = F.R.glu(F.R.expert_linear(F.R.expert_dispatch(x, src, k), w1, off), "silu", act_first=True)
+    off, rows = F.R.expert_plan(idx, w1.shape[0])
+    h = F.R.glu(F.R.expert_linear(F.R.expert_dispatch(x, rows), w1, off), "silu", act_first=True)
     return F.R.expert_combine(F.R.expert_linear(h, w2, off), w, rows)
 
 
