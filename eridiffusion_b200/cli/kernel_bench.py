@@ -1,6 +1,6 @@
 """Per-kernel timing against the library equivalents and the measured roofline.
 
-    python -m eridiffusion_b200.cli.kernel_bench [--what gemm,skinny,attn,elementwise,optim,dequant,narrow,wgrad,small_m,gather_emul,epilogue] [--small]
+    python -m eridiffusion_b200.cli.kernel_bench [--what gemm,skinny,attn,elementwise,optim,dequant,narrow,wgrad,small_m,gather_emul,epilogue,experts,codes] [--small]
 
 Timing: CUDA events on the launching stream, >= 3 warm-up launches, L2 flushed between timed
 launches by writing a 256 MB buffer, median of the timed launches. Roofline denominators come from
@@ -366,6 +366,45 @@ def bench_attn(small):
         print(f"   library SDPA bwd {t_b*1e6:.1f} us {2.5*fl_/t_b/1e12:.0f} TF/s")
 
 
+def bench_experts(small):
+    """Product grouped by expert, forward and both gradients, against a loop of library products over the experts (which needs
+    the numbers of rows on the host)."""
+    bw, fl, tag = peaks()
+    for R_, E, Nn, K in ([(512, 4, 512, 256)] if small else [(64, 16, 5120, 2560), (8192, 16, 4096, 2048), (16384, 8, 5120, 2560)]):
+        share = torch.rand(E, generator=torch.Generator().manual_seed(0)) + 0.25
+        cut = [0, *(share.cumsum(0) / share.sum() * R_).round().int().tolist()]
+        off = torch.tensor(cut, dtype=torch.int32, device="cuda")
+        x, dy = torch.randn(R_, K, device="cuda").bfloat16(), torch.randn(R_, Nn, device="cuda").bfloat16()
+        w = torch.randn(E, Nn, K, device="cuda").mul_(K ** -0.5).bfloat16()
+        lib = F.N.require()
+        y, dx, dw = torch.empty_like(dy), torch.empty_like(x), torch.empty_like(w)
+        ptrs = [t.data_ptr() for t in (x, dy, w, off, y, dx, dw)]
+
+        def run(mode, rows, ld, rows2, ld2, weight, out):
+            F.N.check(lib.eri_expert_gemm(mode, rows, ld, rows2, ld2, weight, ptrs[3], out, R_, E, Nn, K, 0, 0, 0, F.N.stream_ptr()), "expert_gemm")
+        segs = [slice(a, b) for a, b in zip(cut, cut[1:])]
+        pairs = {"forward": (lambda: run(0, ptrs[0], K, None, 0, ptrs[2], ptrs[4]), lambda: [x[s] @ w[e].t() for e, s in enumerate(segs)]),
+                 "dX": (lambda: run(1, ptrs[1], Nn, None, 0, ptrs[2], ptrs[5]), lambda: [dy[s] @ w[e] for e, s in enumerate(segs)]),
+                 "dW": (lambda: run(2, ptrs[0], K, ptrs[1], Nn, None, ptrs[6]), lambda: [dy[s].t() @ x[s] for s in segs])}
+        floor = max(2.0 * R_ * Nn * K / fl, 2.0 * (E * Nn * K + R_ * (Nn + K)) / bw)
+        for name, (ours, library) in pairs.items():
+            t, tl = timeit(ours), timeit(library)
+            print(f"experts {name} rows {R_} E {E} N {Nn} K {K}: {t*1e6:.1f} us, floor {floor*1e6:.1f} us {tag}; library loop {tl*1e6:.1f} us")
+
+
+def bench_codes(small):
+    """Few rows on 4-bit weights against expanding the weight and the bf16 product."""
+    from ..memory import quantize
+    bw, _, tag = peaks()
+    for M, Nn, K in ([(1, 256, 256)] if small else [(1, 15360, 2560), (8, 13824, 5120)]):
+        x = torch.randn(M, K, device="cuda").bfloat16()
+        for kind in ("int4", "nf4"):
+            q = quantize(torch.randn(Nn, K, device="cuda"), kind)
+            t = timeit(lambda: F.linear_4bit(x, q))
+            tx = timeit(lambda: torch.nn.functional.linear(x, q.dequantize(torch.bfloat16)))
+            print(f"{kind} rows {M} N {Nn} K {K}: {t*1e6:.1f} us, floor {q.nbytes()/bw*1e6:.1f} us {tag}; expanded {tx*1e6:.1f} us")
+
+
 def main():
     ap = argparse.ArgumentParser()
     ap.add_argument("--what", default="gemm,elementwise,optim,attn")
@@ -374,7 +413,8 @@ def main():
     for w in a.what.split(","):
         {"gemm": bench_gemm, "skinny": bench_skinny, "elementwise": bench_elementwise, "optim": bench_optim,
          "epilogue": bench_epilogue,
-         "attn": bench_attn, "dequant": bench_dequant, "narrow": bench_narrow, "wgrad": bench_wgrad, "small_m": bench_small_m, "gather_emul": bench_gather_emul}[w](a.small)
+         "attn": bench_attn, "dequant": bench_dequant, "narrow": bench_narrow, "wgrad": bench_wgrad, "small_m": bench_small_m, "gather_emul": bench_gather_emul,
+         "experts": bench_experts, "codes": bench_codes}[w](a.small)
 
 
 if __name__ == "__main__":

@@ -3,7 +3,8 @@ the device, a handful of launches), one per hot kernel:
 
     python -m eridiffusion_b200.cli.profile_target gemm|gemm_lora|rank_stream|attn_fwd|attn_bwd|norm|qknorm|adamw|gemv|
         elementwise|groupnorm|token_route|dequant|attn_masked|small_linear_bwd|slot_reduce|gemm_small_m|gemm_group|
-        gemm_few|attn_wide|attn_bias|norm_rope|norm_rows|column_sums|conv_layout|conv_companions|ema
+        gemm_few|attn_wide|attn_bias|norm_rope|norm_rows|column_sums|conv_layout|conv_companions|ema|
+        experts|expert_exchange|linear_4bit
 
 Meant to be run as ``ncu --set full --clock-control none -k regex:<kernel> -s 2 -c 1 ... python -m
 eridiffusion_b200.cli.profile_target <what>`` after the same command line exited 0 without ncu.
@@ -231,6 +232,35 @@ def main():
         avg = EMA(ParamArena([torch.nn.Parameter(r(112_000_000))]), 0.999)
         for _ in range(iters):
             avg.update()
+    elif what == "experts":
+        # product grouped by expert and both gradients: 8192 rows of uneven experts, 4096 x 2048
+        E, rows, n, k = 16, 8192, 4096, 2048
+        share = torch.rand(E, generator=torch.Generator().manual_seed(0)) + 0.25
+        cut = (share.cumsum(0) / share.sum() * rows).round().int()
+        off = torch.cat([cut.new_zeros(1), cut]).to(dev)
+        x, w, dy = r(rows, k).requires_grad_(), r(E, n, k).requires_grad_(), r(rows, n)
+        for _ in range(iters):
+            torch.autograd.grad(F.expert_linear(x, w, off), (x, w), dy)
+        assert F.kernel_error_check() == {}
+    elif what == "expert_exchange":
+        # 8192 tokens of 2560 channels to six of 64 experts and back, both directions
+        T, E, k, d = 8192, 64, 6, 2560
+        idx, wt = F.expert_route(torch.randn(T, E, device=dev), k)
+        x, y, wt = r(T, d).requires_grad_(), r(T * k, d).requires_grad_(), wt.detach().requires_grad_()
+        dxs, dout = r(T * k, d), r(T, d)
+        for _ in range(iters):
+            plan = F.expert_plan(idx, E)
+            torch.autograd.grad((F.expert_dispatch(x, plan), F.expert_combine(y, wt, plan)), (x, y, wt), (dxs, dout))
+    elif what == "linear_4bit":
+        # one row and the gradient of eight on 4-bit weights (eight weights, larger than L2 together)
+        from ..memory import QuantizedTensor
+        n, k = 15360, 2560
+        qs = [QuantizedTensor("nf4", torch.randint(0, 256, (n * k // 64, 32), dtype=torch.uint8, device=dev),
+                              torch.rand(n * k // 64, device=dev), (n, k), 64) for _ in range(8)]
+        x1, x8, dy = r(1, k), r(8, k).requires_grad_(), r(8, n)
+        for q in qs:
+            F.linear_4bit(x1, q)
+            torch.autograd.grad(F.linear_4bit(x8, q), x8, dy)
     else:
         raise SystemExit(f"unknown target {what}")
     torch.cuda.synchronize()

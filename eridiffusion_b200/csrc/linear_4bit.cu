@@ -656,18 +656,26 @@ int launch4(Args4& p, int dev, cudaStream_t st) {
   const int turns = (pieces + split - 1) / split;
   p.kw = (pieces + turns - 1) / turns;
   // Two CTAs of half the warps share an SM where all rows of x fit: one's prologue and last tiles run beside the other. Shared memory: the
-  // table, every warp's ring of three pieces (two, where that makes room for x), partial sums, x of a pass; fewer rows per pass
-  // (the codes are then read again, from L2) where a long x fits neither way.
-  int per_sm = 2, depth = 3, smem = 0;
-  for (;; per_sm = 1) {
-    p.nw = min_of(kMaxWarps / per_sm / p.kw, tiles);
+  // table, every warp's ring of three pieces (two, where that makes room for x), partial sums, x of a pass. Where x does not
+  // fit, fewer groups of warps (down to half), and where it does not fit then either, fewer rows per pass: the codes are read
+  // again, from L2.
+  int depth = 3, smem = 0;
+  auto fits = [&](int per_sm, int nw) {
+    p.nw = min_of(nw, tiles);
     const int warps = p.kw * p.nw;
     const int fixed = 2 * warps * 8 * kRedRow * 4 + (NF4 ? steps * 32 : 0) + (p.offsets ? 2 * (p.E + 1) * 4 : 0);
     const int room = kSmem4 / per_sm - (per_sm - 1) * 1024 - (NF4 ? kTable : 0) - fixed;
     depth = room - 3 * warps * piece >= want * 2 * p.K ? 3 : 2;
     p.rows = min_of(want, (room - depth * warps * piece) / (2 * p.K));
     smem = fixed + depth * warps * piece + p.rows * 2 * p.K;
-    if (per_sm == 1 || p.rows == want) break;
+    return p.rows == want;
+  };
+  const int most_nw = kMaxWarps / p.kw;
+  int per_sm = 2;
+  if (!fits(2, kMaxWarps / 2 / p.kw)) {
+    per_sm = 1;
+    int nw = most_nw;
+    while (!fits(1, nw) && nw > (most_nw + 1) / 2) --nw;
   }
   if (p.rows < 1) return -100;
   // in the grouped form each row may be a pass of its own
