@@ -181,23 +181,25 @@ __global__ void __launch_bounds__(256) route_bwd_kernel(const T* __restrict__ sc
 // CTA, (3) the CTAs' totals are added over distributed shared memory, (4) the warp walks its piece again and hands out
 // positions. Equal experts inside one group of 32 are found by ballots and ranked by the lanes below, so the order is that of the
 // choices. A piece of at most kHold groups stays in registers between the two walks.
-// Bound by latency: two rounds of loads, four barriers, one read of remote totals. 49152 choices, 64 experts: see kernel table.
+// Bound by instruction issue on its eight SMs (a ballot per bit and group of 32) and, for few choices, by its barriers: 49152
+// choices of 64 experts take 11 us, 14 choices 2.5.
 constexpr int kPlanThreads = 1024, kPlanWarps = kPlanThreads / 32, kHold = 8, kMaxCtas = 8;
 
-__device__ __forceinline__ int load_choice(const void* idx, int wide, long long i, int E) {
+__device__ __forceinline__ int load_choice(const void* idx, int wide, unsigned i, int E) {
   const long long e = wide ? reinterpret_cast<const long long*>(idx)[i] : (long long)reinterpret_cast<const int*>(idx)[i];
   return e >= 0 && e < E ? (int)e : -1;
 }
-__device__ __forceinline__ void load_group(int (&c)[kHold], const void* idx, int wide, long long i0, long long hi, int lane, int E) {
+__device__ __forceinline__ void load_group(int (&c)[kHold], const void* idx, int wide, unsigned i0, unsigned hi, int lane, int E) {
 #pragma unroll
   for (int u = 0; u < kHold; ++u) {
-    const long long i = i0 + 32 * u + lane;
+    const unsigned i = i0 + 32 * u + lane;         // (below 2^32: hi < 2^31)
     c[u] = i < hi ? load_choice(idx, wide, i, E) : -1;
   }
 }
 // Lanes of the warp whose choice is c's (one ballot per bit of an expert's number; lanes without a choice are nobody's).
 __device__ __forceinline__ unsigned same_choice(int c, int bits) {
   unsigned m = __ballot_sync(0xffffffffu, c >= 0);
+#pragma unroll 2
   for (int b = 0; b < bits; ++b) {
     const bool on = (c >> b) & 1;
     const unsigned v = __ballot_sync(0xffffffffu, on);
@@ -221,8 +223,8 @@ __global__ void __launch_bounds__(kPlanThreads) expert_plan_kernel(const void* _
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int rank = ctas > 1 ? (int)cluster_ctarank() : 0;
   const int warps = ctas * kPlanWarps;
-  const long long piece = (((long long)n + warps - 1) / warps + 31) / 32 * 32;
-  const long long lo = min((long long)(rank * kPlanWarps + warp) * piece, (long long)n), hi = min(lo + piece, (long long)n);
+  const unsigned piece = (((unsigned)n + warps - 1) / warps + 31) / 32 * 32;
+  const unsigned lo = (unsigned)min((unsigned long long)(rank * kPlanWarps + warp) * piece, (unsigned long long)n), hi = min(lo + piece, (unsigned)n);
   int* mine = cnt + (size_t)warp * E;
   const int bits = 32 - __clz(E - 1);
   int c[kHold];
@@ -230,7 +232,7 @@ __global__ void __launch_bounds__(kPlanThreads) expert_plan_kernel(const void* _
   load_group(c, idx, wide, lo, hi, lane, E);
   for (int e = lane; e < E; e += 32) mine[e] = 0;
   __syncwarp();
-  for (long long i0 = lo; i0 < hi; i0 += 32 * kHold) {
+  for (unsigned i0 = lo; i0 < hi; i0 += 32 * kHold) {
     if (i0 != lo) load_group(c, idx, wide, i0, hi, lane, E);
 #pragma unroll
     for (int u = 0; u < kHold; ++u) {
@@ -294,12 +296,12 @@ __global__ void __launch_bounds__(kPlanThreads) expert_plan_kernel(const void* _
   }
   __syncthreads();
   const bool held = piece <= 32 * kHold;
-  for (long long i0 = lo; i0 < hi; i0 += 32 * kHold) {
+  for (unsigned i0 = lo; i0 < hi; i0 += 32 * kHold) {
     if (!held) load_group(c, idx, wide, i0, hi, lane, E);
 #pragma unroll
     for (int u = 0; u < kHold; ++u) {
       if (i0 + 32 * u < hi) {
-        const long long i = i0 + 32 * u + lane;
+        const unsigned i = i0 + 32 * u + lane;
         if (!held) same[u] = same_choice(c[u], bits);
         int pos = -1;
         if (c[u] >= 0) pos = first[c[u]] + base[c[u]] + mine[c[u]] + __popc(same[u] & ((1u << lane) - 1u));
