@@ -17,12 +17,10 @@ namespace {
 
 constexpr int kRows = 8, kMaxExperts = 1024;
 
-__constant__ float c_level[2][16] = {
-    {-8.f / 7, -7.f / 7, -6.f / 7, -5.f / 7, -4.f / 7, -3.f / 7, -2.f / 7, -1.f / 7, 0.f, 1.f / 7, 2.f / 7, 3.f / 7, 4.f / 7, 5.f / 7,
-     6.f / 7, 7.f / 7},
-    {-1.0f, -0.6961928009986877f, -0.5250730514526367f, -0.39491748809814453f, -0.28444138169288635f, -0.18477343022823334f,
-     -0.09105003625154495f, 0.0f, 0.07958029955625534f, 0.16093020141124725f, 0.24611230194568634f, 0.33791524171829224f,
-     0.44070982933044434f, 0.5626170039176941f, 0.7229568362236023f, 1.0f}};
+__constant__ float c_nf4[16] = {-1.0f, -0.6961928009986877f, -0.5250730514526367f, -0.39491748809814453f, -0.28444138169288635f,
+                                -0.18477343022823334f, -0.09105003625154495f, 0.0f, 0.07958029955625534f, 0.16093020141124725f,
+                                0.24611230194568634f, 0.33791524171829224f, 0.44070982933044434f, 0.5626170039176941f, 0.7229568362236023f,
+                                1.0f};
 
 struct Segment {
   int e, rows;        // rows of this CTA from row r on: 0 = another CTA's, -1 = row r belongs to no expert
@@ -54,6 +52,9 @@ __device__ __forceinline__ Segment segment_of(const int* offsets, int E, int R, 
 // The reduction is split over the `kw` warps of a group, `nw` groups take 16 weight rows each. A warp copies the pieces of codes that
 // it alone reads (four steps of 16 rows) asynchronously into a ring of its own, across the tiles of a persistent CTA, so that no
 // warp waits for another but for the sum of a tile: partial sums meet in shared memory and are added in warp order.
+// Bound by instruction issue (about 120 per warp and 1024 codes: decoding 48, ring copies 20, sums, barriers and x the rest), not by the
+// 23 bytes per cycle and SM that memory delivers. us in a row of launches: one row 15360 x 2560 NF4 12.4 (22 MB, 5 of them before and
+// behind the loop), 75776 x 2560 36.8 (3.0 TB/s), eight rows 13824 x 5120 int4 20. Twelve rows of 9 experts of 5120 x 2560 24.6.
 constexpr int kU = 4;                       // steps of a piece
 constexpr int kMaxWarps = 20, kMaxSplit = 10;     // warps of an SM, warps that share a tile
 constexpr int kTable = 256 * 32 * 4;        // bytes of the NF4 table
@@ -229,7 +230,7 @@ __device__ __forceinline__ Pass pass_of(int i, const int* bound, const int* pass
 }
 __device__ __forceinline__ void build_table(uint8_t* table) {       // four lanes' copies of a pair at a time
   for (int i = threadIdx.x; i < 256 * 8; i += blockDim.x) {
-    const uint32_t v = half2_bits(c_level[1][(i >> 3) & 15], c_level[1][i >> 7]);
+    const uint32_t v = half2_bits(c_nf4[(i >> 3) & 15], c_nf4[i >> 7]);
     reinterpret_cast<uint4*>(table)[i] = make_uint4(v, v, v, v);
   }
 }
@@ -424,7 +425,8 @@ __global__ void __launch_bounds__(kMaxWarps * 32, 1) linear_4bit_kernel(const Ar
 // place its largest magnitude at 2^8, and when a later one would pass 2^15 the sums are scaled down with it (rare). Values down to
 // 2^-22 of the largest keep all their bits, the rest is off by 2^-33 of it.
 // A CTA owns one piece of columns (256, or 128 with blocks of 32) and a range of weight rows; its warps take every kDgWarps-th 16 rows, their
-// sums meet in shared memory in warp order, and the ranges' planes are added in order by the kernel below.
+// sums meet in shared memory in warp order, and the ranges' planes are added in order by the kernel below. us: 13824 x 5120 int4, eight
+// rows, 22 and 4 for the planes (160 with one thread per eight columns and the products in 32 bits).
 constexpr int kDgWarps = 16, kDgDepth = 3, kDgRows = 2048;        // kDgRows: most weight rows of a range (their dy is in shared memory)
 
 template <bool NF4>
