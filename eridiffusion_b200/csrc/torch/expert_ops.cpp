@@ -260,7 +260,10 @@ OptT linear_4bit(const Tensor& x, const Tensor& codes, const Tensor& scale_, con
   const Tensor bias = contig(opt(bias_));
   Tensor offsets = opt(offsets_);
   same_device("linear_4bit", x, {&codes, &scale_, &offsets, &bias});
-  if (!codes.is_contiguous() || !al16(codes)) return OptT();
+  const int64_t weights = experts * N * x.size(-1);
+  TORCH_CHECK_VALUE(codes.numel() * 2 == weights && scale_.numel() * block == weights, "linear_4bit: ", codes.numel(), " bytes of codes and ",
+                    scale_.numel(), " scales for ", weights, " weights in blocks of ", block);
+  if (codes.scalar_type() != at::kByte || !codes.is_contiguous() || !al16(codes)) return OptT();
   if (offsets.defined()) offsets = int32(offsets);
   const Tensor scale = contig(scale_.scalar_type() == at::kFloat ? scale_ : scale_.to(at::kFloat));
   const int64_t K = x.size(-1);

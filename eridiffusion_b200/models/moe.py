@@ -124,7 +124,7 @@ def moe_linear(x: torch.Tensor, scores: torch.Tensor, bank: ExpertBank, k: int =
     the experts some token uses (at most ``resident`` of them, chosen by ``select_topk_global``)."""
     allowed = select_topk_global(scores, resident) if resident else None
     idx, w = route_tokens(scores, k, allowed)
-    y = _moe_grouped(x, idx, w, scores.shape[-1], bank, allowed)
+    y = _moe_grouped(x, idx, w, scores.shape[-1], bank, resident)
     if y is not None:
         return y
     out = None
@@ -138,33 +138,52 @@ def moe_linear(x: torch.Tensor, scores: torch.Tensor, bank: ExpertBank, k: int =
     return out.to(x.dtype)
 
 
-def _moe_grouped(x, idx, w, total: int, bank: ExpertBank, allowed):
+def _moe_grouped(x, idx, w, total: int, bank: ExpertBank, resident):
     """``moe_linear`` as one grouped product on the GPU; None where that does not apply."""
     if not (x.is_cuda and x.dtype == torch.bfloat16 and x.dim() == 2 and x.shape[0] > 0 and F.get_backend() == "fused"):
         return None
-    ids = [i for i in (range(total) if allowed is None else sorted(allowed)) if i in bank.experts]
+    ids = [i for i in range(total) if i in bank.experts]
     if not ids:
         return None
-    weight = bank.stacked(ids)
-    if weight is None:
-        # int8 codes are expanded per expert: only those that some token uses
+    first = bank.experts[ids[0]]
+    if tuple(first.shape) != (first.shape[0], x.shape[1]):
+        return None
+    weight, rows = None, x.shape[0] * idx.shape[1]
+    if not isinstance(first, QuantizedTensor) or (first.kind in ("int4", "nf4") and rows <= F.CODES_EXPERT_ROWS):
+        weight = bank.stacked(ids)           # all that are present, whatever is allowed: stacked once
+        if weight is None or (weight.data if isinstance(weight, QuantizedTensor) else weight).device != x.device:
+            return None
+    else:
+        # codes are expanded for many rows: only the experts that some token uses, a few at a time
         used = set(idx.flatten().tolist())
         ids = [i for i in ids if i in used]
-        expanded = [dequantize_to_bf16(bank.experts[i]) for i in ids]
-        if not ids or any(e.dim() != 2 or e.shape != expanded[0].shape for e in expanded):
+        codes = [bank.experts[i] for i in ids]
+        if not ids or any(not isinstance(q, QuantizedTensor) or tuple(q.shape) != tuple(first.shape) or q.data.device != x.device for q in codes):
             return None
-        weight = torch.stack(expanded)
-    stack_device = weight.data.device if isinstance(weight, QuantizedTensor) else weight.device
-    if stack_device != x.device or weight.shape[-1] != x.shape[1]:
-        return None
-    if len(ids) != total:                # the experts' places in the stack; an absent expert adds nothing
+    if len(ids) != total:                    # the experts' places in the bank; an absent expert adds nothing
         place = torch.full((total,), -1, dtype=torch.int64)
         place[ids] = torch.arange(len(ids))
         idx = place.to(x.device)[idx]
     plan = F.expert_plan(idx, len(ids))
-    rows = F.expert_dispatch(x, plan)
+    xs = F.expert_dispatch(x, plan)
     if isinstance(weight, QuantizedTensor):
-        y = F.linear_4bit(rows, weight, plan.offsets)
+        y = F.linear_4bit(xs, weight, plan.offsets)
+    elif weight is not None:
+        y = F.expert_linear(xs, weight, plan.offsets)
     else:
-        y = F.expert_linear(rows, weight, plan.offsets)
+        n, k = first.shape
+        step = max(1, min(len(ids), resident or len(ids), _EXPANDED_BYTES // (2 * n * k)))
+        y = None
+        for a in range(0, len(ids), step):
+            part = codes[a:a + step]
+            weight = torch.empty(len(part), n, k, dtype=torch.bfloat16, device=x.device)
+            for out, q in zip(weight, part):
+                w_bf16 = dequantize(q, torch.bfloat16, out=out)
+                if w_bf16 is not out:
+                    out.copy_(w_bf16)
+            rows_y = F.expert_linear(xs, weight, plan.offsets[a:a + len(part) + 1])        # zeros for the rows of other experts
+            y = rows_y if y is None else y + rows_y
     return F.expert_combine(y, w, plan)
+
+
+_EXPANDED_BYTES = 1 << 30        # most bytes of expanded experts at a time

@@ -1040,12 +1040,12 @@ def expert_linear(x, w, offsets):
 
 # Most rows that are multiplied with the codes themselves; above, the weight is expanded once and meets the matrix kernels. Widest row:
 # x of a pass, the rings and the tables share an SM's memory.
-_CODES_ROWS, _CODES_EXPERT_ROWS, _CODES_WIDTH = 8, 64, 16384
+CODES_ROWS, CODES_EXPERT_ROWS, _CODES_WIDTH = 8, 64, 16384
 
 
 def on_codes(x, q) -> bool:
     """Whether ``linear_4bit`` multiplies x with the codes of the dense weight ``q`` themselves."""
-    return (q.kind in ("int4", "nf4") and len(q.shape) == 2 and _native_ok(x) and x.numel() <= _CODES_ROWS * q.shape[1]
+    return (q.kind in ("int4", "nf4") and len(q.shape) == 2 and _native_ok(x) and x.numel() <= CODES_ROWS * q.shape[1]
             and q.shape[1] <= _CODES_WIDTH and q.shape[1] % q.block == 0 and q.block % 32 == 0)
 
 
@@ -1074,7 +1074,7 @@ def linear_4bit(x, q, offsets=None, bias=None):
     if x.shape[-1:] != (K,):
         raise ValueError(f"linear_4bit: x {tuple(x.shape)} for a weight of shape {tuple(shape)}")
     native = _native_ok(x, bias)
-    if native and x.numel() <= (_CODES_EXPERT_ROWS if experts else _CODES_ROWS) * K and E <= _MAX_EXPERTS and K <= _CODES_WIDTH \
+    if native and x.numel() <= (CODES_EXPERT_ROWS if experts else CODES_ROWS) * K and E <= _MAX_EXPERTS and K <= _CODES_WIDTH \
             and K % q.block == 0 and q.block % 32 == 0 and Nn > 0:
         y = N.ops().linear_4bit(x, q.data, q.scale, offsets, bias, E, Nn, q.block, nf4)
         if y is not None:

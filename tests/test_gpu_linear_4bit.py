@@ -172,7 +172,7 @@ def test_many_experts_per_cta(E, N, K, block, kind):
     y = F.linear_4bit(x, q, off)
     (dx,) = torch.autograd.grad(y, x, dy)
     we = _weight64(q)[torch.repeat_interleave(torch.arange(E), torch.tensor(counts)).cuda()]
-    xd, dd, expanded = x.detach().double(), dy.double(), R > F._CODES_EXPERT_ROWS       # (the first case: 77 rows)
+    xd, dd, expanded = x.detach().double(), dy.double(), R > F.CODES_EXPERT_ROWS       # (the first case: 77 rows)
     _near(y.detach(), torch.einsum("rk,rnk->rn", xd, we), torch.einsum("rk,rnk->rn", xd.abs(), we.abs()), K, expanded)
     _near(dx, torch.einsum("rn,rnk->rk", dd, we), torch.einsum("rn,rnk->rk", dd.abs(), we.abs()), N, expanded)
 
@@ -188,3 +188,14 @@ def test_long_rows_take_several_passes(kind):
     w = _weight64(q)
     _near(y.detach(), x.detach().double() @ w.t(), x.detach().double().abs() @ w.abs().t(), 16384)
     _near(dx, dy.double() @ w, dy.double().abs() @ w.abs(), 50)
+
+
+def test_codes_of_another_size_are_refused():
+    g = _gen(19)
+    q = _random(g, "int4", (64, 128), 64)
+    x = _mk(g, 2, 128)
+    for data, scale in ((q.data[:-1], q.scale), (q.data, q.scale[:-1])):
+        with pytest.raises(ValueError):
+            F.linear_4bit(x, QuantizedTensor("int4", data, scale, (64, 128), 64))
+    with pytest.raises(ValueError):
+        F.linear_4bit(x, QuantizedTensor("int4", q.data.cpu(), q.scale, (64, 128), 64))

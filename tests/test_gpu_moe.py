@@ -54,6 +54,34 @@ def test_bank(T, E, N, K, k, resident, missing, kind):
     assert len(bank) == E - len(missing) and {i for i, _ in bank.fetch_topk_bf16(range(E))} == set(weights)
 
 
+@pytest.mark.parametrize("kind", ["q8", "nf4"])
+def test_expanded_a_few_at_a_time(kind, monkeypatch):
+    from eridiffusion_b200.models import moe
+    g = torch.Generator(device="cuda").manual_seed(3)
+    bank = ExpertBank(kind)
+    for e in range(7):
+        bank.insert(e, _mk(g, 128, 256, std=0.05))
+    x, scores = _mk(g, 200, 256), torch.randn(200, 7, device="cuda", generator=g)
+    whole = moe_linear(x, scores, bank, k=2)
+    monkeypatch.setattr(moe, "_EXPANDED_BYTES", 3 * 2 * 128 * 256)
+    assert torch.equal(moe_linear(x, scores, bank, k=2), whole)          # three at a time: the same sums
+    monkeypatch.undo()
+    assert all(b.data.untyped_storage().nbytes() == b.data.numel() for b in bank.experts.values() if kind == "nf4")     # nothing was stacked
+
+
+def test_bank_with_changing_residents_is_stacked_once():
+    g = torch.Generator(device="cuda").manual_seed(5)
+    bank = ExpertBank("none")
+    for e in range(6):
+        bank.insert(e, _mk(g, 64, 128))
+    x = _mk(g, 30, 128)
+    moe_linear(x, torch.randn(30, 6, device="cuda", generator=g), bank, k=2, resident=2)
+    held = bank._stack[2]
+    for _ in range(3):
+        moe_linear(x, torch.randn(30, 6, device="cuda", generator=g), bank, k=2, resident=3)
+        assert bank._stack[2] is held and all(e.untyped_storage().data_ptr() == held.untyped_storage().data_ptr() for e in bank.experts.values())
+
+
 def test_bank_follows_a_replaced_expert():
     g = torch.Generator(device="cuda").manual_seed(1)
     bank = ExpertBank("none")
