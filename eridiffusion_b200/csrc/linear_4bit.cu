@@ -152,13 +152,21 @@ struct PieceRing {
       const int s0 = piece * kU, si = w.ratio == 1 ? s0 + t : (s0 + t) / w.ratio;
       const int left = w.N - tile * 16;                          // weight rows from here on
       const uint8_t* q = src;
+      if (WHOLE && left >= 16) {                                // nothing to leave out
 #pragma unroll
-      for (int i = 0; i < kCopies; ++i, q += (32 / kChunks) * w.k_bytes)
-        if ((WHOLE || piece * kRow + lane % kChunks * 16 < w.k_bytes) && (left >= 16 || i * (32 / kChunks) + row < left)) copy16(dst + put + i * 512, q);
+        for (int i = 0; i < kCopies; ++i, q += (32 / kChunks) * w.k_bytes) copy16(dst + put + i * 512, q);
+        const float* s = s_src + si;
+        copy4(s_dst + put, s);
+        copy4(s_dst + put + 128, s + 8 * w.spr);
+      } else {
 #pragma unroll
-      for (int h = 0; h < 2; ++h)
-        if (WHOLE || s0 + t < w.K / STEP)
-          copy4(s_dst + put + 128 * h, s_src + (left >= 16 || g + 8 * h < left ? 8 * h : left - 1 - g) * w.spr + si);
+        for (int i = 0; i < kCopies; ++i, q += (32 / kChunks) * w.k_bytes)
+          if ((WHOLE || piece * kRow + lane % kChunks * 16 < w.k_bytes) && (left >= 16 || i * (32 / kChunks) + row < left)) copy16(dst + put + i * 512, q);
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+          if (WHOLE || s0 + t < w.K / STEP)
+            copy4(s_dst + put + 128 * h, s_src + (left >= 16 || g + 8 * h < left ? 8 * h : left - 1 - g) * w.spr + si);
+      }
       src += kRow;
       if (++piece == p_hi) {
         piece = p_lo;
