@@ -977,8 +977,8 @@ def expert_route(scores, k, allowed=None, normalize=True):
     if allowed is not None:
         if allowed.dtype != torch.bool or allowed.shape != (E,):
             raise ValueError(f"expert_route: allowed must be a boolean [{E}], got {tuple(allowed.shape)} {allowed.dtype}")
-    if scores.is_cuda and _BACKEND == "fused" and scores.dtype in (torch.float32, torch.bfloat16) and T > 0 and E <= _MAX_EXPERTS \
-            and k <= _MAX_TOP:
+    if scores.is_cuda and _BACKEND == "fused" and scores.dtype in (torch.float32, torch.bfloat16) and 0 < T < 2 ** 31 \
+            and E <= _MAX_EXPERTS and k <= _MAX_TOP:
         return tuple(N.ops().expert_route(scores, allowed, k, normalize))
     _same_device("expert_route", scores, allowed)
     return R.expert_route(scores, k, allowed, normalize)
@@ -1032,7 +1032,8 @@ def expert_linear(x, w, offsets):
     _check_offsets("expert_linear", offsets, E)
     if x.dtype != w.dtype:
         raise ValueError(f"expert_linear: x {x.dtype}, w {w.dtype}")
-    if _native_ok(x, w) and E <= _MAX_EXPERTS and Nn % 8 == 0 and K % 8 == 0 and Nn > 0 and K > 0 and x.shape[0] < 2 ** 31:
+    if _native_ok(x, w) and E <= _MAX_EXPERTS and Nn % 8 == 0 and K % 8 == 0 and 0 < Nn < 2 ** 31 and 0 < K < 2 ** 31 \
+            and x.shape[0] < 2 ** 30:
         return N.ops().expert_linear(x, w, offsets, 0, _ACCUM_INTO_GRAD)
     _same_device("expert_linear", x, w, offsets)
     return R.expert_linear(x, w, offsets)
