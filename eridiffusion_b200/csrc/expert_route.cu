@@ -395,68 +395,134 @@ __global__ void __launch_bounds__(256) expert_gather_kernel(const bf16* __restri
   }
 }
 
-// One CTA per token: dout[t] is read once and meets the token's k rows; the dot products are added in lane and warp order. 8192 tokens, six
-// rows of 2560: 104 us, 5.3 TB/s of reads and writes in equal parts (five or ten warps per token, two vectors per lane or 64
-// registers a thread for more CTAs: 111 to 122 us).
-constexpr int kGbThreads = 128, kGbTop = 8;
-__global__ void __launch_bounds__(kGbThreads) expert_gather_bwd_kernel(const bf16* __restrict__ dout, long long ldo,
-                                                                       const bf16* __restrict__ y, long long ldy,
-                                                                       const int* __restrict__ rows, const float* __restrict__ w,
-                                                                       const int* __restrict__ live, bf16* __restrict__ dy,
-                                                                       float* __restrict__ dw, int tokens, int k, int n_rows, int D) {
-  __shared__ float part[kGbThreads / 32][kGbTop];
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const long long t = blockIdx.x;
-  if (t < tokens) {
-    for (int j0 = 0; j0 < k; j0 += kGbTop) {
-      float dot[kGbTop], f[kGbTop];
-      int r[kGbTop];
+// dy[rows[t, j]] = w[t, j] dout[t] and dw[t, j] = <dout[t], y[rows[t, j]]>. `split` warps share a token, each 256 columns at a time: dout[t] and up to
+// TOP of its rows come through a ring that the warp fills a piece ahead with asynchronous copies, across its tokens, so that reads do not
+// wait for the stores of the piece before. The dot products are added in lane and warp order. Bound by DRAM with several rows per token, by
+// issue with one. us, tokens x columns, rows per token: 8192 x 2560, 6: 89 to 98 (5.6 to 6.1 TB/s of reads and writes in equal parts; a CTA per
+// token that loads into registers 105), 16384 x 2560, 2: 76 (139), 30000 x 1280, 1: 77 (159), 512 x 2560, 6: 7.5 (8.8). Three pieces:
+// 4096 x 4096, 8: 94 instead of 100, but 512 x 2560 8.5; 16 warps per SM instead of 24: 16384 x 2560 84.
+constexpr int kGbWarps = 8, kGbDepth = 2, kGbCols = 256, kGbRow = kGbCols * 2;
+__device__ __forceinline__ void copy16(uint32_t dst, const void* src) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+}
+// Sums of TOP values over the warp, TOP - 1 + log2(32 / TOP) shuffles: lane l is left with the sum of value l / (32 / TOP).
+template <int TOP>
+__device__ __forceinline__ float warp_sums(float (&v)[TOP], int lane) {
 #pragma unroll
-      for (int u = 0; u < kGbTop; ++u) {
-        dot[u] = 0.f;
-        r[u] = j0 + u < k ? rows[t * k + j0 + u] : -1;
-        if (r[u] >= n_rows) r[u] = -1;
-        f[u] = r[u] >= 0 ? w[t * k + j0 + u] : 0.f;
-      }
-      for (int c = threadIdx.x * 8; c < D; c += kGbThreads * 8) {
-        float g[8];
-        unpack8(*reinterpret_cast<const bf16x8*>(dout + t * ldo + c), g);
-        bf16x8 v[kGbTop];
-        if (dw) {
+  for (int n = TOP / 2, o = 16; n >= 1; n /= 2, o /= 2) {
+    const bool up = lane & o;
 #pragma unroll
-          for (int u = 0; u < kGbTop; ++u)
-            if (r[u] >= 0) v[u] = *reinterpret_cast<const bf16x8*>(y + (long long)r[u] * ldy + c);
+    for (int i = 0; i < n; ++i) {
+      const float keep = up ? v[i + n] : v[i], give = up ? v[i] : v[i + n];
+      v[i] = keep + __shfl_xor_sync(0xffffffffu, give, o);
+    }
+  }
+#pragma unroll
+  for (int o = 16 / TOP; o >= 1; o /= 2) v[0] += __shfl_xor_sync(0xffffffffu, v[0], o);
+  return v[0];
+}
+template <int TOP>
+__global__ void __launch_bounds__(kGbWarps * 32, 3) expert_gather_bwd_kernel(const bf16* __restrict__ dout, long long ldo,
+                                                                             const bf16* __restrict__ y, long long ldy,
+                                                                             const int* __restrict__ rows, const float* __restrict__ w,
+                                                                             const int* __restrict__ live, bf16* __restrict__ dy,
+                                                                             float* __restrict__ dw, int tokens, int k, int n_rows, int D,
+                                                                             int split) {
+  extern __shared__ __align__(16) uint8_t gb_ring[];
+  __shared__ float part[2][kGbWarps][TOP];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, groups = (blockDim.x >> 5) / split, group = warp / split, wk = warp % split;
+  const int piece = (min(k, TOP) + 1) * kGbRow, ring_bytes = kGbDepth * piece;
+  const uint8_t* ring = gb_ring + warp * ring_bytes + lane * 16;
+  const uint32_t dst = smem_u32(ring);
+  const int c0 = wk * kGbCols, c_step = split * kGbCols;
+  const long long first = blockIdx.x + (long long)group * gridDim.x, stride = (long long)gridDim.x * groups;
+  // Row and weight of choice j0 + u in lane u; absent ones are -1.
+  auto row_of = [&](long long t, int j0) {
+    int r = -1;
+    if (t < tokens && lane < TOP && j0 + lane < k) r = rows[t * k + j0 + lane];
+    return r < n_rows ? r : -1;
+  };
+  auto weight_of = [&](long long t, int j0) { return t < tokens && lane < TOP && j0 + lane < k ? w[t * k + j0 + lane] : 0.f; };
+  // the piece to fetch next: token, first of its TOP choices, columns
+  long long ft = first;
+  int fj = 0, fc = c0, fr = row_of(ft, 0), put = 0, get = 0;
+  auto fetch = [&] {
+    if (ft < tokens) {
+      const int c = fc + lane * 8;
+      const bool on = c < D;
+      if (on) copy16(dst + put, dout + ft * ldo + c);
+      if (dw) {
+#pragma unroll
+        for (int u = 0; u < TOP; ++u) {
+          const int r = __shfl_sync(0xffffffffu, fr, u);
+          if (on && r >= 0) copy16(dst + put + (u + 1) * kGbRow, y + r * ldy + c);
         }
+      }
+      fc += c_step;
+      if (fc >= D) {
+        fc = c0;
+        fj += TOP;
+        if (fj >= k) { fj = 0; ft += stride; }
+        fr = row_of(ft, fj);
+      }
+    }
+    put = put + piece == ring_bytes ? 0 : put + piece;
+    asm volatile("cp.async.commit_group;" ::: "memory");      // also an empty group, so that groups count pieces
+  };
 #pragma unroll
-        for (int u = 0; u < kGbTop; ++u)
-          if (r[u] >= 0) {
+  for (int i = 0; i < kGbDepth - 1; ++i) fetch();
+  int buf = 0, next_r = row_of(first, 0);
+  float next_f = weight_of(first, 0);
+  for (long long t = first; t < tokens; t += stride) {
+    for (int j0 = 0; j0 < k; j0 += TOP) {
+      const int mr = next_r;
+      const float mf = next_f;
+      const bool last = j0 + TOP >= k;
+      next_r = row_of(last ? t + stride : t, last ? 0 : j0 + TOP);          // a round ahead
+      next_f = weight_of(last ? t + stride : t, last ? 0 : j0 + TOP);
+      float dot[TOP];
+#pragma unroll
+      for (int u = 0; u < TOP; ++u) dot[u] = 0.f;
+      for (int c = c0 + lane * 8; c - lane * 8 < D; c += c_step) {
+        fetch();                          // into the piece read last; a lane reads what it copied itself
+        asm volatile("cp.async.wait_group %0;" ::"n"(kGbDepth - 1) : "memory");
+        const uint8_t* p = ring + get;
+        get = get + piece == ring_bytes ? 0 : get + piece;
+        float g[8];
+        unpack8(*reinterpret_cast<const bf16x8*>(p), g);                    // whatever there is behind the last column: not used
+#pragma unroll
+        for (int u = 0; u < TOP; ++u) {
+          const int r = __shfl_sync(0xffffffffu, mr, u);
+          const float f = __shfl_sync(0xffffffffu, mf, u);
+          if (r >= 0 && c < D) {
             if (dw) {
               float a[8];
-              unpack8(v[u], a);
+              unpack8(*reinterpret_cast<const bf16x8*>(p + (u + 1) * kGbRow), a);
 #pragma unroll
               for (int q = 0; q < 8; ++q) dot[u] = fmaf(g[q], a[q], dot[u]);
             }
             if (dy) {
               float o[8];
 #pragma unroll
-              for (int q = 0; q < 8; ++q) o[q] = f[u] * g[q];
-              *reinterpret_cast<bf16x8*>(dy + (long long)r[u] * D + c) = pack8(o);
+              for (int q = 0; q < 8; ++q) o[q] = f * g[q];
+              *reinterpret_cast<bf16x8*>(dy + (long long)r * D + c) = pack8(o);
             }
           }
+        }
       }
       if (dw) {
-#pragma unroll
-        for (int u = 0; u < kGbTop; ++u) {
-          const float s = warp_sum(dot[u]);
-          if (lane == 0) part[warp][u] = s;
+        const int u = lane / (32 / TOP);
+        float sum = warp_sums<TOP>(dot, lane);
+        const bool mine = lane % (32 / TOP) == 0;
+        if (split > 1) {
+          if (mine) part[buf][warp][u] = sum;
+          asm volatile("bar.sync %0, %1;" ::"r"(1 + group), "r"(split * 32) : "memory");
+          sum = 0.f;
+          if (wk == 0 && mine)
+            for (int q = 0; q < split; ++q) sum += part[buf][warp + q][u];
+          buf ^= 1;       // the next round writes the other half; the barrier there is behind these reads
         }
-        __syncthreads();
-        if (threadIdx.x < kGbTop && j0 + threadIdx.x < k) {
-          float s = 0.f;
-          for (int q = 0; q < kGbThreads / 32; ++q) s += part[q][threadIdx.x];
-          dw[t * k + j0 + threadIdx.x] = s;
-        }
-        __syncthreads();
+        if (wk == 0 && mine && j0 + u < k) dw[t * k + j0 + u] = sum;
       }
     }
   }
@@ -465,9 +531,31 @@ __global__ void __launch_bounds__(kGbThreads) expert_gather_bwd_kernel(const bf1
     const long long rest = (long long)(n_rows - from) * (D >> 3);
     bf16x8 z;
     z.u = make_uint4(0, 0, 0, 0);
-    for (long long it = (long long)blockIdx.x * kGbThreads + threadIdx.x; it < rest; it += (long long)gridDim.x * kGbThreads)
+    for (long long it = (long long)blockIdx.x * blockDim.x + threadIdx.x; it < rest; it += (long long)gridDim.x * blockDim.x)
       *reinterpret_cast<bf16x8*>(dy + (long long)from * D + it * 8) = z;
   }
+}
+template <int TOP>
+int gather_bwd(const bf16* dout, long long ldo, const bf16* y, long long ldy, const int* rows, const float* w, const int* live, bf16* dy,
+               float* dw, int tokens, int k, int n_rows, int D, cudaStream_t st) {
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return -2;
+  static int sms[64] = {};
+  if (!sms[dev]) {
+    int n = 0;
+    if (cudaFuncSetAttribute(expert_gather_bwd_kernel<TOP>, cudaFuncAttributeMaxDynamicSharedMemorySize, kGbWarps * kGbDepth * (TOP + 1) * kGbRow) != cudaSuccess ||
+        cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess)
+      return -3;
+    sms[dev] = n;
+  }
+  // as many warps per token as it has pieces of 256 columns, or pieces per warp alike
+  const int chunks = (D + kGbCols - 1) / kGbCols, turns = (chunks + kGbWarps - 1) / kGbWarps, split = (chunks + turns - 1) / turns;
+  const int groups = kGbWarps / split, warps = groups * split, smem = warps * kGbDepth * ((k < TOP ? k : TOP) + 1) * kGbRow;
+  const int by_smem = 225 * 1024 / (smem + 2048), by_regs = 3 * kGbWarps / warps, per_sm = by_smem < by_regs ? by_smem : by_regs;
+  const long long most = ((long long)tokens + groups - 1) / groups, ctas = (long long)per_sm * sms[dev];
+  expert_gather_bwd_kernel<TOP><<<(unsigned)(most < ctas ? most : ctas), warps * 32, smem, st>>>(dout, ldo, y, ldy, rows, w, live, dy, dw, tokens,
+                                                                                                  k, n_rows, D, split);
+  return (int)cudaGetLastError();
 }
 
 template <typename T>
@@ -582,9 +670,10 @@ int eri_expert_gather(const void* y, long long ldy, const int* rows, const float
 int eri_expert_gather_bwd(const void* dout, long long ldo, const void* y, long long ldy, const int* rows, const float* w, const int* live,
                           void* dy, float* dw, int tokens, int k, int n_rows, int D, void* stream) {
   if (!dims_ok(tokens, k, n_rows, D) || ldo % 8 || ldy % 8 || (((uintptr_t)dout | (uintptr_t)y | (uintptr_t)dy) & 15)) return -1;
-  expert_gather_bwd_kernel<<<(unsigned)tokens, kGbThreads, 0, (cudaStream_t)stream>>>((const bf16*)dout, ldo, (const bf16*)y, ldy, rows, w,
-                                                                                       live, (bf16*)dy, dw, tokens, k, n_rows, D);
-  return (int)cudaGetLastError();
+#define ERI_GATHER_BWD(TOP) \
+  gather_bwd<TOP>((const bf16*)dout, ldo, (const bf16*)y, ldy, rows, w, live, (bf16*)dy, dw, tokens, k, n_rows, D, (cudaStream_t)stream)
+  return k == 1 ? ERI_GATHER_BWD(1) : k == 2 ? ERI_GATHER_BWD(2) : k <= 4 ? ERI_GATHER_BWD(4) : ERI_GATHER_BWD(8);
+#undef ERI_GATHER_BWD
 }
 
 }  // extern "C"

@@ -120,7 +120,8 @@ def test_plan_of_one_expert_only():
         assert none.offsets.tolist() == [0] * 6 and (none.rows == -1).all()
 
 
-@pytest.mark.parametrize("T,k,E,D", [(1, 1, 1, 8), (7, 2, 32, 640), (65, 9, 12, 136), (300, 17, 40, 1288), (1000, 4, 8, 72)])
+@pytest.mark.parametrize("T,k,E,D", [(1, 1, 1, 8), (7, 2, 32, 640), (65, 9, 12, 136), (300, 17, 40, 1288), (1000, 4, 8, 72), (5000, 1, 9, 264), (4000, 3, 9, 72),
+                                     (1500, 8, 64, 2312), (700, 9, 16, 4104)])       # with more tokens than the kernels hold at a time
 @pytest.mark.parametrize("padded", [False, True])
 def test_dispatch_and_combine(T, k, E, D, padded):
     g = _gen(T + k + D)
