@@ -52,9 +52,9 @@ __device__ __forceinline__ Segment segment_of(const int* offsets, int E, int R, 
 // The reduction is split over the `kw` warps of a group, `nw` groups take 16 weight rows each. A warp copies the pieces of codes that
 // it alone reads (four steps of 16 rows) asynchronously into a ring of its own, across the tiles of a persistent CTA, so that no
 // warp waits for another but for the sum of a tile: partial sums meet in shared memory and are added in warp order.
-// Bound by instruction issue (about 120 per warp and 1024 codes: decoding 48, ring copies 20, sums, barriers and x the rest), not by the
-// 23 bytes per cycle and SM that memory delivers. us in a row of launches: one row 15360 x 2560 NF4 12.4 (22 MB, 5 of them before and
-// behind the loop), 75776 x 2560 36.8 (3.0 TB/s), eight rows 13824 x 5120 int4 20. Twelve rows of 9 experts of 5120 x 2560 24.6.
+// Bound by instruction issue (about 115 per warp and 1024 codes: decoding 48, ring copies 15, sums, barriers and x the rest), not by the
+// 23 bytes per cycle and SM that memory delivers. us in a row of launches: one row 15360 x 2560 NF4 12.2 (22 MB, 5 of them before and
+// behind the loop), 75776 x 2560 36.4 (3.0 TB/s; 34.8 with the codes in L2), eight rows 13824 x 5120 int4 20. Twelve rows of 9 experts of 5120 x 2560 24.6.
 constexpr int kU = 4;                       // steps of a piece
 constexpr int kMaxWarps = 20, kMaxSplit = 10;     // warps of an SM, warps that share a tile
 constexpr int kTable = 256 * 32 * 4;        // bytes of the NF4 table
