@@ -169,7 +169,8 @@ def quantize(w: torch.Tensor, kind="int8", block=64) -> QuantizedTensor:
         q = torch.round(wf / s).clamp(-127, 127).to(torch.int8)
         return QuantizedTensor(kind, q, s.squeeze(-1), shape, 0)
     flat = wf.reshape(-1, block)
-    s = flat.abs().amax(dim=1, keepdim=True).clamp_min(1e-12)
+    scale = flat.abs().amax(dim=1).clamp_min(1e-12)
+    s = scale.unsqueeze(1)
     if kind == "int4":
         q = (torch.round(flat / s * 7.0).clamp(-8, 7) + 8).to(torch.uint8)
     elif kind == "nf4":
@@ -177,7 +178,7 @@ def quantize(w: torch.Tensor, kind="int8", block=64) -> QuantizedTensor:
     else:
         raise ValueError(kind)
     packed = (q[:, 0::2] | (q[:, 1::2] << 4)).contiguous()
-    return QuantizedTensor(kind, packed, s.squeeze(1), shape, block)
+    return QuantizedTensor(kind, packed, scale, shape, block)
 
 
 def _dequantize_native(q: QuantizedTensor, out=None):

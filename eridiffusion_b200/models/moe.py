@@ -14,7 +14,9 @@ one resident in bf16 at a time) and token-routed feed-forward experts.
 """
 from __future__ import annotations
 
+import collections
 import enum
+import sys
 
 import torch
 
@@ -43,7 +45,7 @@ class ExpertBank:
     def __init__(self, kind: QuantKind | str = QuantKind.Q8):
         self.kind = QuantKind(kind)
         self.experts: dict[int, object] = {}
-        self._stack = None              # (ids, their entries, stacked weight)
+        self._stack = None              # (ids, where their entries lie, stacked weight)
 
     def insert(self, expert_id: int, weight):
         """``weight``: a tensor (quantised on insertion) or an already quantised weight."""
@@ -60,34 +62,68 @@ class ExpertBank:
         """[(id, bf16 weight)] for the ids that are present, in the order asked."""
         return [(int(i), dequantize_to_bf16(self.experts[int(i)])) for i in ids if int(i) in self.experts]
 
-
     def stacked(self, ids):
         """The weights of the present experts ``ids`` as one [len(ids), N, K] tensor or, for 4-bit codes, one ``QuantizedTensor`` of
-        that shape. The bank's entries become views of it, so that nothing is held twice; it is made again when an entry
-        is replaced. None where they are of different shapes, kinds or devices, or stored as int8."""
+        that shape. The entries are moved into it (the same tensor objects on other memory), so that nothing is held twice and a
+        change of an entry is a change of the stack. None where someone else holds an entry's memory (a caller's tensor, whose
+        changes in place the bank has to follow), where an entry records gradients, or where the entries are of different shapes,
+        kinds or devices, or not stored as bf16, int4 or NF4."""
         ids = tuple(ids)
         entries = [self.experts[i] for i in ids]
-        if self._stack is not None and self._stack[0] == ids and all(a is b for a, b in zip(self._stack[1], entries)):
+        if self._stack is not None and self._stack[0] == ids and self._stack[1] == _places(entries):
             return self._stack[2]
         self._stack = None
-        first = entries[0]
+        parts = _stackable(entries)
+        if parts is None or not _sole_holders([t for part in parts for t in part]):
+            return None
+        joined = [torch.stack(part) for part in parts]
+        for whole, part in zip(joined, parts):
+            for t, home in zip(part, whole):
+                t.data = home
+        first, weight = entries[0], joined[0]
         if isinstance(first, QuantizedTensor):
-            key = [(e.kind, tuple(e.shape), e.block, e.data.device) if isinstance(e, QuantizedTensor) else None for e in entries]
-            if first.kind not in ("int4", "nf4") or len(first.shape) != 2 or any(k != key[0] for k in key):
-                return None
-            data, scale = torch.cat([e.data for e in entries]), torch.cat([e.scale for e in entries])
-            weight = QuantizedTensor(first.kind, data, scale, (len(ids), *first.shape), first.block)
-            per = first.data.shape[0]
-            views = [QuantizedTensor(first.kind, data[i * per:(i + 1) * per], scale[i * per:(i + 1) * per], first.shape, first.block)
-                     for i in range(len(ids))]
-        else:
-            if any(isinstance(e, QuantizedTensor) or e.dim() != 2 or e.shape != first.shape or e.device != first.device for e in entries):
-                return None
-            weight = torch.stack([e.to(torch.bfloat16) for e in entries])
-            views = list(weight.unbind(0))
-        self.experts.update(zip(ids, views))
-        self._stack = (ids, views, weight)
+            weight = QuantizedTensor(first.kind, joined[0].flatten(0, 1), joined[1].flatten(), (len(ids), *first.shape), first.block)
+        self._stack = (ids, _places(entries), weight)
         return weight
+
+
+def _places(entries):
+    """What tells whether entries still lie where a stack that is alive has them."""
+    return [(e.kind, e.block, tuple(e.shape), e.data.data_ptr(), e.data.shape, e.scale.data_ptr(), e.scale.shape)
+            if isinstance(e, QuantizedTensor) else (e.data_ptr(), e.shape, e.stride(), e.dtype, e.requires_grad) for e in entries]
+
+
+def _holders(t):
+    """Holders of a tensor's memory: tensors (one more for the storage object made here), and references to that object."""
+    storage = t.untyped_storage()
+    return storage._cdata, torch._C._storage_Use_Count(storage._cdata), sys.getrefcount(storage)
+
+
+def _sole_holders(tensors) -> bool:
+    """Whether nothing but these tensors holds their memory, so that it may be given up when they are moved."""
+    here = collections.Counter(t.untyped_storage()._cdata for t in tensors)
+    _, alone, refs = _holders(torch.empty(1))
+    return all((users, r) == (alone - 1 + here[key], refs) for key, users, r in map(_holders, tensors))
+
+
+def _stackable(entries):
+    """The tensors to stack, entry by entry: [weights] or [codes, scales]; None where they do not go together."""
+    first = entries[0]
+    if isinstance(first, QuantizedTensor):
+        if first.kind not in ("int4", "nf4") or len(first.shape) != 2 \
+                or any(not isinstance(e, QuantizedTensor) or (e.kind, tuple(e.shape), e.block) != (first.kind, tuple(first.shape), first.block) for e in entries):
+            return None
+        parts = [[e.data for e in entries], [e.scale for e in entries]]
+    else:
+        if any(isinstance(e, QuantizedTensor) or e.dim() != 2 or e.dtype != torch.bfloat16 for e in entries):
+            return None
+        parts = [list(entries)]
+    for part in parts:
+        t0 = part[0]
+        if len({id(t) for t in part}) != len(part) or any(
+                t.shape != t0.shape or t.dtype != t0.dtype or t.device != t0.device or not t.is_contiguous() or t.requires_grad for t in part):
+            return None
+    return parts
 
 
 def select_topk_global(scores_or_total, k: int):
@@ -148,18 +184,18 @@ def _moe_grouped(x, idx, w, total: int, bank: ExpertBank, resident):
     first = bank.experts[ids[0]]
     if tuple(first.shape) != (first.shape[0], x.shape[1]):
         return None
-    weight, rows = None, x.shape[0] * idx.shape[1]
-    if not isinstance(first, QuantizedTensor) or (first.kind in ("int4", "nf4") and rows <= F.CODES_EXPERT_ROWS):
+    weight, entries = None, None
+    if not isinstance(first, QuantizedTensor) or (first.kind in ("int4", "nf4") and x.shape[0] * idx.shape[1] <= F.CODES_EXPERT_ROWS):
         weight = bank.stacked(ids)           # all that are present, whatever is allowed: stacked once
-        if weight is None or (weight.data if isinstance(weight, QuantizedTensor) else weight).device != x.device:
-            return None
-    else:
-        # codes are expanded for many rows: only the experts that some token uses, a few at a time
+    if weight is None:
+        # codes of many rows, and weights that are not stacked: only the experts that some token uses, a few at a time
         used = set(idx.flatten().tolist())
         ids = [i for i in ids if i in used]
-        codes = [bank.experts[i] for i in ids]
-        if not ids or any(not isinstance(q, QuantizedTensor) or tuple(q.shape) != tuple(first.shape) or q.data.device != x.device for q in codes):
+        entries = [bank.experts[i] for i in ids]
+        if not ids or any(tuple(e.shape) != tuple(first.shape) for e in entries):
             return None
+    if any(_device(e) != x.device for e in entries or (weight,)):
+        return None
     if len(ids) != total:                    # the experts' places in the bank; an absent expert adds nothing
         place = torch.full((total,), -1, dtype=torch.int64)
         place[ids] = torch.arange(len(ids))
@@ -175,15 +211,26 @@ def _moe_grouped(x, idx, w, total: int, bank: ExpertBank, resident):
         step = max(1, min(len(ids), resident or len(ids), _EXPANDED_BYTES // (2 * n * k)))
         y = None
         for a in range(0, len(ids), step):
-            part = codes[a:a + step]
-            weight = torch.empty(len(part), n, k, dtype=torch.bfloat16, device=x.device)
-            for out, q in zip(weight, part):
-                w_bf16 = dequantize(q, torch.bfloat16, out=out)
-                if w_bf16 is not out:
-                    out.copy_(w_bf16)
-            rows_y = F.expert_linear(xs, weight, plan.offsets[a:a + len(part) + 1])        # zeros for the rows of other experts
+            part = entries[a:a + step]
+            rows_y = F.expert_linear(xs, _expanded(part), plan.offsets[a:a + len(part) + 1])        # zeros for the rows of other experts
             y = rows_y if y is None else y + rows_y
     return F.expert_combine(y, w, plan)
+
+
+def _device(weight):
+    return weight.data.device if isinstance(weight, QuantizedTensor) else weight.device
+
+
+def _expanded(entries):
+    """bf16 weights of some experts, [len(entries), N, K]."""
+    if not all(isinstance(e, QuantizedTensor) for e in entries):
+        return torch.stack([dequantize_to_bf16(e) for e in entries])
+    weight = torch.empty(len(entries), *entries[0].shape, dtype=torch.bfloat16, device=entries[0].data.device)
+    for out, q in zip(weight, entries):
+        w_bf16 = dequantize(q, torch.bfloat16, out=out)
+        if w_bf16 is not out:
+            out.copy_(w_bf16)
+    return weight
 
 
 _EXPANDED_BYTES = 1 << 30        # most bytes of expanded experts at a time

@@ -1,0 +1,108 @@
+"""Stacking of an expert bank: which entries may be moved, and that every holder of an entry goes on seeing the bank's values."""
+import copy
+import gc
+
+import pytest
+import torch
+
+from eridiffusion_b200.memory import QuantizedTensor, quantize
+from eridiffusion_b200.models.moe import ExpertBank
+
+BF = torch.bfloat16
+
+
+def _weights(n, shape=(24, 64)):
+    g = torch.Generator().manual_seed(n)
+    return [torch.randn(*shape, generator=g).to(BF) for _ in range(n)]
+
+
+def test_changes_of_a_callers_tensor_are_seen():
+    ws = _weights(3)
+    bank = ExpertBank("none")
+    for i, w in enumerate(ws):
+        bank.insert(i, w)
+    bank.stacked(range(3))
+    ws[1].add_(1.0)
+    assert all(torch.equal(a, b) for (_, a), b in zip(bank.fetch_topk_bf16(range(3)), ws))
+    assert bank.stacked(range(3)) is None
+
+
+def test_entries_that_nobody_else_holds_are_moved():
+    ws = _weights(3)
+    bank = ExpertBank("none")
+    for i, w in enumerate(ws):
+        bank.insert(i, w.clone())
+    entries = [bank.experts[i] for i in range(3)]
+    whole = bank.stacked(range(3))
+    assert whole is bank.stacked(range(3)) and torch.equal(whole, torch.stack(ws))
+    assert all(bank.experts[i] is e and e.untyped_storage().data_ptr() == whole.untyped_storage().data_ptr() for i, e in enumerate(entries))
+    entries[2].mul_(2.0)                                       # a change of an entry is a change of the stack
+    assert torch.equal(bank.stacked(range(3))[2], ws[2] * 2)
+
+
+def test_codes_of_a_callers_weight_stay_the_callers():
+    qs = [quantize(w, "nf4") for w in _weights(3)]
+    bank = ExpertBank("nf4")
+    for i, q in enumerate(qs):
+        bank.insert(i, q)
+    want = [q.dequantize(torch.float32) for q in qs]
+    whole = bank.stacked(range(3))
+    assert torch.equal(whole.dequantize(torch.float32), torch.stack(want))
+    qs[0].scale.mul_(2.0)                                      # through the caller's object, after the move
+    assert torch.equal(bank.stacked(range(3)).dequantize(torch.float32)[0], want[0] * 2)
+    held = qs[1].data.view(-1)                                 # another holder of the memory: no further move
+    qs[2].data = qs[2].data.clone()
+    assert bank.stacked(range(3)) is None
+    held.zero_()
+    assert torch.equal(bank.experts[1].dequantize(torch.float32), torch.full((24, 64), -1.0) * qs[1].scale.repeat_interleave(64).view(24, 64))
+
+
+def test_a_replaced_expert_is_stacked_anew():
+    ws = _weights(4)
+    bank = ExpertBank("none")
+    for i in range(3):
+        bank.insert(i, ws[i].clone())
+    bank.stacked(range(3))
+    bank.insert(1, ws[3].clone())
+    assert torch.equal(bank.stacked(range(3)), torch.stack([ws[0], ws[3], ws[2]]))
+    bank.experts[0].data = ws[1].clone()
+    assert torch.equal(bank.stacked(range(3)), torch.stack([ws[1], ws[3], ws[2]]))
+
+
+@pytest.mark.parametrize("what", ["twice", "dtype", "shape", "gradient", "strides", "kinds", "int8"])
+def test_what_is_not_stacked(what):
+    a, b = _weights(2, (64, 64))
+    bank = ExpertBank("none")
+    bank.insert(0, a.clone())
+    bank.insert(1, b.clone())
+    if what == "twice":
+        bank.experts[1] = bank.experts[0]
+    elif what == "dtype":
+        bank.experts[1] = b.float()
+    elif what == "shape":
+        bank.experts[1] = b[:32].clone()
+    elif what == "gradient":
+        bank.experts[1].requires_grad_()
+    elif what == "strides":
+        bank.experts[1].t_()
+    else:
+        bank.experts[1] = quantize(b, "nf4" if what == "kinds" else "int8")
+        if what == "int8":
+            bank.experts[0] = quantize(a, "int8")
+    before = {i: (e.dequantize(torch.float32) if isinstance(e, QuantizedTensor) else e.detach().clone()) for i, e in bank.experts.items()}
+    assert bank.stacked((0, 1)) is None
+    for i, e in bank.experts.items():
+        now = e.dequantize(torch.float32) if isinstance(e, QuantizedTensor) else e
+        assert now.dtype == before[i].dtype and torch.equal(now, before[i])
+
+
+def test_copies_of_a_stacked_bank_are_their_own():
+    bank = ExpertBank("none")
+    for i, w in enumerate(_weights(2)):
+        bank.insert(i, w.clone())
+    whole = bank.stacked((0, 1)).clone()
+    other = copy.deepcopy(bank)
+    other.experts[0].zero_()
+    gc.collect()
+    assert torch.equal(bank.stacked((0, 1)), whole)
+    assert other.stacked((0, 1))[0].count_nonzero() == 0 and torch.equal(other.stacked((0, 1))[1], whole[1])

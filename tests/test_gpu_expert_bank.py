@@ -1,0 +1,75 @@
+"""``moe_linear`` on an ``ExpertBank`` whose entries change, are held elsewhere, or are first used in unusual places."""
+import pytest
+import torch
+
+from eridiffusion_b200.memory import QuantizedTensor
+from eridiffusion_b200.models.moe import ExpertBank, moe_linear
+
+pytestmark = pytest.mark.gpu
+BF = torch.bfloat16
+E, N, K = 6, 136, 192
+
+
+def _mk(g, *s, std=1.0):
+    return (torch.randn(*s, device="cuda", generator=g) * std).to(BF)
+
+
+def _weight64(e):
+    return (e.dequantize(torch.float32) if isinstance(e, QuantizedTensor) else e).detach().double()
+
+
+def _near(y, x, scores, bank, k=2):
+    """Against 64 bits: expert outputs and their sum are rounded to bf16 (2^-8 of themselves each); expanded weights 2^-8, levels of
+    few rows 2^-11 of themselves; sums over K in 32 bits."""
+    top, idx = torch.sort(scores.double(), dim=-1, descending=True, stable=True)
+    w = torch.softmax(top[:, :k], -1)
+    ref, err = 0, 0
+    for j in range(k):
+        for e, q in bank.experts.items():
+            hit = (idx[:, j] == e).double()[:, None] * w[:, j:j + 1]
+            we, xd = _weight64(q), x.detach().double()
+            p = xd @ we.t()
+            ref = ref + hit * p
+            err = err + hit * (p.abs() * 2 ** -8 + (xd.abs() @ we.abs().t()) * (K * 2 ** -23 + (2 ** -8 if isinstance(q, QuantizedTensor) else 0)))
+    assert y.dtype == BF and ((y.double() - ref).abs() <= (ref.abs() * 2 ** -8 + err) * 1.01 + 1e-30).all()
+
+
+def _bank(kind, g, held=None):
+    bank = ExpertBank(kind)
+    for e in range(E):
+        w = _mk(g, N, K, std=0.07)
+        if held is not None:
+            held.append(w)
+        bank.insert(e, w)
+    return bank
+
+
+def _inputs(g, T):
+    return _mk(g, T, K), torch.randn(T, E, device="cuda", generator=g)
+
+
+@pytest.mark.parametrize("T", [1, 5, 300])
+def test_changes_of_the_callers_weights_are_followed(T):
+    g = torch.Generator(device="cuda").manual_seed(T)
+    held = []
+    bank = _bank("none", g, held)
+    x, scores = _inputs(g, T)
+    for _ in range(3):
+        _near(moe_linear(x, scores, bank), x, scores, bank)
+        assert all(torch.equal(bank.experts[i], w) for i, w in enumerate(held))
+        for w in held:
+            w.copy_(_mk(g, N, K, std=0.07))
+
+
+@pytest.mark.parametrize("T", [1, 5, 300])
+@pytest.mark.parametrize("kind", ["none", "nf4"])
+def test_changes_of_entries_are_followed(kind, T):
+    g = torch.Generator(device="cuda").manual_seed(T + 1)
+    bank = _bank(kind, g)
+    x, scores = _inputs(g, T)
+    entries = list(bank.experts.values())
+    for _ in range(3):
+        _near(moe_linear(x, scores, bank), x, scores, bank)
+        for e in entries:
+            (e.scale if kind == "nf4" else e).mul_(1.5)
+        assert all(bank.experts[i] is e for i, e in enumerate(entries))
