@@ -46,6 +46,7 @@ class ExpertBank:
         self.kind = QuantKind(kind)
         self.experts: dict[int, object] = {}
         self._stack = None              # (ids, where their entries lie, stacked weight)
+        self._fixed = False             # a captured graph reads the entries where they lie
 
     def insert(self, expert_id: int, weight):
         """``weight``: a tensor (quantised on insertion) or an already quantised weight."""
@@ -60,18 +61,28 @@ class ExpertBank:
 
     def fetch_topk_bf16(self, ids):
         """[(id, bf16 weight)] for the ids that are present, in the order asked."""
+        self._fix_if_captured()
         return [(int(i), dequantize_to_bf16(self.experts[int(i)])) for i in ids if int(i) in self.experts]
+
+    def _fix_if_captured(self) -> bool:
+        """Whether the current stream captures; the entries then stay where they lie, for the replays."""
+        captured = _capturing(next((_device(e) for e in self.experts.values()), None))
+        self._fixed |= captured
+        return captured
 
     def stacked(self, ids):
         """The weights of the present experts ``ids`` as one [len(ids), N, K] tensor or, for 4-bit codes, one ``QuantizedTensor`` of
         that shape. The entries are moved into it (the same tensor objects on other memory), so that nothing is held twice and a
         change of an entry is a change of the stack. None where someone else holds an entry's memory (a caller's tensor, whose
-        changes in place the bank has to follow), where an entry records gradients, or where the entries are of different shapes,
+        changes in place the bank has to follow), where an entry records gradients, where a captured graph reads the entries (a call
+        under capture moves nothing: the copies would only be recorded), or where the entries are of different shapes,
         kinds or devices, or not stored as bf16, int4 or NF4."""
         ids = tuple(ids)
         entries = [self.experts[i] for i in ids]
         if self._stack is not None and self._stack[0] == ids and self._stack[1] == _places(entries):
             return self._stack[2]
+        if self._fix_if_captured() or self._fixed:
+            return None
         self._stack = None
         parts = _stackable(entries)
         if parts is None or not _sole_holders([t for part in parts for t in part]):
@@ -184,13 +195,15 @@ def _moe_grouped(x, idx, w, total: int, bank: ExpertBank, resident):
     first = bank.experts[ids[0]]
     if tuple(first.shape) != (first.shape[0], x.shape[1]):
         return None
-    weight, entries = None, None
+    weight, entries, captured = None, None, bank._fix_if_captured()
     if not isinstance(first, QuantizedTensor) or (first.kind in ("int4", "nf4") and x.shape[0] * idx.shape[1] <= F.CODES_EXPERT_ROWS):
         weight = bank.stacked(ids)           # all that are present, whatever is allowed: stacked once
     if weight is None:
-        # codes of many rows, and weights that are not stacked: only the experts that some token uses, a few at a time
-        used = set(idx.flatten().tolist())
-        ids = [i for i in ids if i in used]
+        # codes of many rows, and weights that are not stacked: a few at a time, and only the experts that some token uses
+        # (all of them under capture, where nothing can be read back)
+        if not captured:
+            used = set(idx.flatten().tolist())
+            ids = [i for i in ids if i in used]
         entries = [bank.experts[i] for i in ids]
         if not ids or any(tuple(e.shape) != tuple(first.shape) for e in entries):
             return None
@@ -215,6 +228,13 @@ def _moe_grouped(x, idx, w, total: int, bank: ExpertBank, resident):
             rows_y = F.expert_linear(xs, _expanded(part), plan.offsets[a:a + len(part) + 1])        # zeros for the rows of other experts
             y = rows_y if y is None else y + rows_y
     return F.expert_combine(y, w, plan)
+
+
+def _capturing(device) -> bool:
+    if device is None or device.type != "cuda":
+        return False
+    with torch.cuda.device(device):
+        return torch.cuda.is_current_stream_capturing()
 
 
 def _device(weight):

@@ -106,3 +106,37 @@ def test_copies_of_a_stacked_bank_are_their_own():
     gc.collect()
     assert torch.equal(bank.stacked((0, 1)), whole)
     assert other.stacked((0, 1))[0].count_nonzero() == 0 and torch.equal(other.stacked((0, 1))[1], whole[1])
+
+
+@pytest.mark.parametrize("first", ["stacked", "fetched"])
+def test_nothing_moves_once_a_graph_reads_the_bank(first, monkeypatch):
+    from eridiffusion_b200.models import moe
+    bank = ExpertBank("none")
+    for i, w in enumerate(_weights(3)):
+        bank.insert(i, w.clone())
+    at = [bank.experts[i].data_ptr() for i in range(3)]
+    monkeypatch.setattr(moe, "_capturing", lambda device: True)
+    if first == "stacked":
+        assert bank.stacked(range(3)) is None
+    else:
+        bank.fetch_topk_bf16([0])
+    monkeypatch.undo()
+    assert bank.stacked(range(3)) is None                      # a replay reads the entries where they were
+    assert [bank.experts[i].data_ptr() for i in range(3)] == at
+
+
+def test_a_stack_made_before_a_capture_is_kept_by_it(monkeypatch):
+    from eridiffusion_b200.models import moe
+    ws = _weights(4)
+    bank = ExpertBank("none")
+    for i in range(3):
+        bank.insert(i, ws[i].clone())
+    whole = bank.stacked(range(3))
+    at = whole.data_ptr()
+    monkeypatch.setattr(moe, "_capturing", lambda device: True)
+    bank._fix_if_captured()
+    assert bank.stacked(range(3)) is whole
+    monkeypatch.undo()
+    del whole
+    bank.insert(3, ws[3].clone())
+    assert bank.stacked(range(4)) is None and [bank.experts[i].data_ptr() for i in range(3)] == [at + i * 24 * 64 * 2 for i in range(3)]

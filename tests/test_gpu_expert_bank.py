@@ -73,3 +73,48 @@ def test_changes_of_entries_are_followed(kind, T):
         for e in entries:
             (e.scale if kind == "nf4" else e).mul_(1.5)
         assert all(bank.experts[i] is e for i, e in enumerate(entries))
+
+
+def _capture(fn):
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = fn()
+    return graph, out
+
+
+@pytest.mark.parametrize("called_before", [False, True])
+@pytest.mark.parametrize("T", [1, 5, 300])
+@pytest.mark.parametrize("kind", ["none", "q8", "nf4"])
+def test_captured_call(kind, T, called_before):
+    """The first call of a bank may be captured: replays follow the entries, also after eager calls and other allocations."""
+    g = torch.Generator(device="cuda").manual_seed(T + 2)
+    bank = _bank(kind, g)
+    x, scores = _inputs(g, T)
+    if called_before:
+        moe_linear(x, scores, bank)
+    at = [(e.data if isinstance(e, QuantizedTensor) else e).data_ptr() for e in bank.experts.values()]
+    graph, y = _capture(lambda: moe_linear(x, scores, bank))
+    for i in range(3):
+        junk = [torch.full((E * N * K,), float("nan"), device="cuda", dtype=BF) for _ in range(4)]
+        x.copy_(_mk(g, T, K))
+        scores.copy_(torch.randn(T, E, device="cuda", generator=g))
+        for e in bank.experts.values():
+            (e.scale if isinstance(e, QuantizedTensor) else e).mul_(1.25)
+        graph.replay()
+        _near(y, x, scores, bank)
+        _near(moe_linear(x, scores, bank), x, scores, bank)
+        del junk
+    assert [(e.data if isinstance(e, QuantizedTensor) else e).data_ptr() for e in bank.experts.values()] == at
+
+
+def test_fetched_under_capture_then_called():
+    g = torch.Generator(device="cuda").manual_seed(4)
+    bank = _bank("none", g)
+    x, scores = _inputs(g, 5)
+    out = torch.empty(N, K, device="cuda", dtype=BF)
+    graph, _ = _capture(lambda: out.copy_(bank.fetch_topk_bf16([2])[0][1] * 2))
+    _near(moe_linear(x, scores, bank), x, scores, bank)
+    junk = [torch.full((N * K,), float("nan"), device="cuda", dtype=BF) for _ in range(2 * E)]
+    graph.replay()
+    assert torch.equal(out, bank.experts[2] * 2)
+    del junk
