@@ -17,6 +17,7 @@ from __future__ import annotations
 import collections
 import enum
 import sys
+import threading
 
 import torch
 
@@ -41,11 +42,15 @@ def dequantize_to_bf16(qw) -> torch.Tensor:
     return dequantize(qw, torch.bfloat16) if isinstance(qw, QuantizedTensor) else qw.to(torch.bfloat16)
 
 
+_MOVING = threading.Lock()
+
+
 class ExpertBank:
     def __init__(self, kind: QuantKind | str = QuantKind.Q8):
         self.kind = QuantKind(kind)
         self.experts: dict[int, object] = {}
         self._stack = None              # (ids, where their entries lie, stacked weight)
+        self._streams = set()           # whose memory stacks are
         self._fixed = False             # a captured graph reads the entries where they lie
 
     def insert(self, expert_id: int, weight):
@@ -62,13 +67,23 @@ class ExpertBank:
     def fetch_topk_bf16(self, ids):
         """[(id, bf16 weight)] for the ids that are present, in the order asked."""
         self._fix_if_captured()
-        return [(int(i), dequantize_to_bf16(self.experts[int(i)])) for i in ids if int(i) in self.experts]
+        return [(int(i), dequantize_to_bf16(self._here(self.experts[int(i)]))) for i in ids if int(i) in self.experts]
 
     def _fix_if_captured(self) -> bool:
         """Whether the current stream captures; the entries then stay where they lie, for the replays."""
         captured = _capturing(next((_device(e) for e in self.experts.values()), None))
         self._fixed |= captured
         return captured
+
+    def _here(self, weight):
+        """``weight``, an entry or a stack, for the current stream: memory of another stream's stack may not be given to others
+        before this stream has read it."""
+        if self._streams and _device(weight).type == "cuda":
+            stream = torch.cuda.current_stream(_device(weight))
+            if self._streams != {stream.cuda_stream}:
+                for t in (weight.data, weight.scale) if isinstance(weight, QuantizedTensor) else (weight,):
+                    t.record_stream(stream)
+        return weight
 
     def stacked(self, ids):
         """The weights of the present experts ``ids`` as one [len(ids), N, K] tensor or, for 4-bit codes, one ``QuantizedTensor`` of
@@ -77,7 +92,11 @@ class ExpertBank:
         changes in place the bank has to follow), where an entry records gradients, where a captured graph reads the entries (a call
         under capture moves nothing: the copies would only be recorded), or where the entries are of different shapes,
         kinds or devices, or not stored as bf16, int4 or NF4."""
-        ids = tuple(ids)
+        with _MOVING:
+            weight = self._stacked(tuple(ids))
+        return None if weight is None else self._here(weight)
+
+    def _stacked(self, ids):
         entries = [self.experts[i] for i in ids]
         if self._stack is not None and self._stack[0] == ids and self._stack[1] == _places(entries):
             return self._stack[2]
@@ -88,6 +107,10 @@ class ExpertBank:
         if parts is None or not _sole_holders([t for part in parts for t in part]):
             return None
         joined = [torch.stack(part) for part in parts]
+        if joined[0].is_cuda:
+            # every stream finds the stack filled, and nothing reads the old memory any more when it is given back
+            torch.cuda.synchronize(joined[0].device)
+            self._streams.add(torch.cuda.current_stream(joined[0].device).cuda_stream)
         for whole, part in zip(joined, parts):
             for t, home in zip(part, whole):
                 t.data = home
@@ -204,7 +227,7 @@ def _moe_grouped(x, idx, w, total: int, bank: ExpertBank, resident):
         if not captured:
             used = set(idx.flatten().tolist())
             ids = [i for i in ids if i in used]
-        entries = [bank.experts[i] for i in ids]
+        entries = [bank._here(bank.experts[i]) for i in ids]
         if not ids or any(tuple(e.shape) != tuple(first.shape) for e in entries):
             return None
     if any(_device(e) != x.device for e in entries or (weight,)):

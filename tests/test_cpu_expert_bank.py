@@ -140,3 +140,31 @@ def test_a_stack_made_before_a_capture_is_kept_by_it(monkeypatch):
     del whole
     bank.insert(3, ws[3].clone())
     assert bank.stacked(range(4)) is None and [bank.experts[i].data_ptr() for i in range(3)] == [at + i * 24 * 64 * 2 for i in range(3)]
+
+
+def test_memory_of_another_streams_stack_is_recorded(monkeypatch):
+    """A stack is ready for every stream when it is made, and what another stream reads of it is not given to others before."""
+    from types import SimpleNamespace
+    from eridiffusion_b200.models import moe
+
+    class OnGpu(torch.Tensor):
+        is_cuda = True
+        log = []
+
+        def record_stream(self, stream):
+            self.log.append(stream.cuda_stream)
+    bank, device, now = ExpertBank("none"), torch.device("cuda", 0), [7]
+    for i, w in enumerate(_weights(2)):
+        bank.insert(i, w.clone())
+    synced = []
+    monkeypatch.setattr(torch, "stack", lambda ts: torch.cat([t[None] for t in ts]).as_subclass(OnGpu))
+    monkeypatch.setattr(torch.cuda, "synchronize", lambda d: synced.append([bank.experts[i].data_ptr() for i in range(2)]))
+    monkeypatch.setattr(torch.cuda, "current_stream", lambda d=None: SimpleNamespace(cuda_stream=now[0]))
+    monkeypatch.setattr(moe, "_device", lambda w: device)
+    monkeypatch.setattr(moe, "_capturing", lambda d: False)
+    before = [bank.experts[i].data_ptr() for i in range(2)]
+    whole = bank.stacked((0, 1))
+    assert synced == [before] and [bank.experts[i].data_ptr() for i in range(2)] != before       # filled before the old memory goes
+    assert OnGpu.log == []
+    now[0] = 8
+    assert bank.stacked((0, 1)) is whole and OnGpu.log == [8] and len(synced) == 1

@@ -118,3 +118,51 @@ def test_fetched_under_capture_then_called():
     graph.replay()
     assert torch.equal(out, bank.experts[2] * 2)
     del junk
+
+
+def _junk(n=3 * E):
+    return [torch.full((N * K,), float("nan"), device="cuda", dtype=BF) for _ in range(n)] + [torch.full((E * N * K,), float("nan"), device="cuda", dtype=BF)]
+
+
+@pytest.mark.parametrize("kind", ["none", "nf4"])
+def test_first_call_on_another_stream(kind):
+    """The first call waits on a busy stream: what the bank's own stream allocates and writes meanwhile is not its weights, and a third
+    stream finds them without waiting for the first one."""
+    g = torch.Generator(device="cuda").manual_seed(6)
+    bank = _bank(kind, g)
+    want = [_weight64(e).clone() for e in bank.experts.values()]
+    x, scores = _inputs(g, 5)
+    busy, other = torch.cuda.Stream(), torch.cuda.Stream()
+    torch.cuda.synchronize()
+    with torch.cuda.stream(busy):
+        torch.cuda._sleep(40_000_000)
+        y = moe_linear(x, scores, bank)
+    junk = _junk()
+    with torch.cuda.stream(other):
+        z = moe_linear(x, scores, bank)
+    torch.cuda.synchronize()
+    assert all(torch.equal(_weight64(e), w) for e, w in zip(bank.experts.values(), want))
+    _near(y, x, scores, bank)
+    _near(z, x, scores, bank)
+    del junk
+
+
+@pytest.mark.parametrize("kind", ["none", "nf4"])
+def test_bank_dropped_while_another_stream_reads_it(kind):
+    g = torch.Generator(device="cuda").manual_seed(8)
+    bank = _bank(kind, g)
+    x, scores = _inputs(g, 5)
+    first = torch.cuda.Stream()
+    torch.cuda.synchronize()
+    with torch.cuda.stream(first):
+        y = moe_linear(x, scores, bank)
+    torch.cuda.synchronize()
+    torch.cuda._sleep(40_000_000)
+    z = moe_linear(x, scores, bank)
+    bank.experts.clear()
+    del bank
+    with torch.cuda.stream(first):
+        junk = _junk()
+    torch.cuda.synchronize()
+    assert torch.equal(y, z)
+    del junk
