@@ -89,9 +89,9 @@ class ExpertBank:
         """The weights of the present experts ``ids`` as one [len(ids), N, K] tensor or, for 4-bit codes, one ``QuantizedTensor`` of
         that shape. The entries are moved into it (the same tensor objects on other memory), so that nothing is held twice and a
         change of an entry is a change of the stack. None where someone else holds an entry's memory (a caller's tensor, whose
-        changes in place the bank has to follow), where an entry records gradients, where a captured graph reads the entries (a call
-        under capture moves nothing: the copies would only be recorded), or where the entries are of different shapes,
-        kinds or devices, or not stored as bf16, int4 or NF4."""
+        changes in place the bank has to follow), where an entry records gradients or was made in inference mode, where a captured
+        graph reads the entries (a call under capture moves nothing: the copies would only be recorded), or where the entries
+        are of different shapes, kinds or devices, or not stored as bf16, int4 or NF4."""
         with _MOVING:
             weight = self._stacked(tuple(ids))
         return None if weight is None else self._here(weight)
@@ -106,7 +106,8 @@ class ExpertBank:
         parts = _stackable(entries)
         if parts is None or not _sole_holders([t for part in parts for t in part]):
             return None
-        joined = [torch.stack(part) for part in parts]
+        with torch.inference_mode(False), torch.no_grad():       # it outlives this call and its mode
+            joined = [torch.stack(part) for part in parts]
         if joined[0].is_cuda:
             # every stream finds the stack filled, and nothing reads the old memory any more when it is given back
             torch.cuda.synchronize(joined[0].device)
@@ -155,7 +156,8 @@ def _stackable(entries):
     for part in parts:
         t0 = part[0]
         if len({id(t) for t in part}) != len(part) or any(
-                t.shape != t0.shape or t.dtype != t0.dtype or t.device != t0.device or not t.is_contiguous() or t.requires_grad for t in part):
+                t.shape != t0.shape or t.dtype != t0.dtype or t.device != t0.device or not t.is_contiguous() or t.requires_grad
+                or t.is_inference() for t in part):
             return None
     return parts
 

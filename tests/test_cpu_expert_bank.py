@@ -168,3 +168,18 @@ def test_memory_of_another_streams_stack_is_recorded(monkeypatch):
     assert OnGpu.log == []
     now[0] = 8
     assert bank.stacked((0, 1)) is whole and OnGpu.log == [8] and len(synced) == 1
+
+
+def test_a_stack_made_in_inference_mode_is_an_ordinary_tensor():
+    bank, made_inside = ExpertBank("none"), ExpertBank("none")
+    for i, w in enumerate(_weights(2)):
+        bank.insert(i, w.clone())
+    with torch.inference_mode():
+        whole = bank.stacked((0, 1))
+        for i, w in enumerate(_weights(2)):
+            made_inside.insert(i, w.clone())
+        assert made_inside.stacked((0, 1)) is None             # they cannot be saved for a backward pass, as stack or alone
+    assert not whole.is_inference() and not any(e.is_inference() for e in bank.experts.values())
+    x = torch.ones(1, 64, dtype=BF, requires_grad=True)
+    (x @ bank.stacked((0, 1))[0].t()).sum().backward()
+    assert x.grad is not None

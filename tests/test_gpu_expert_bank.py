@@ -166,3 +166,20 @@ def test_bank_dropped_while_another_stream_reads_it(kind):
     torch.cuda.synchronize()
     assert torch.equal(y, z)
     del junk
+
+
+@pytest.mark.parametrize("T", [5, 300])
+@pytest.mark.parametrize("inserted_inside", [False, True])
+@pytest.mark.parametrize("kind", ["none", "nf4"])
+def test_training_after_a_call_in_inference_mode(kind, inserted_inside, T):
+    g = torch.Generator(device="cuda").manual_seed(10)
+    with torch.inference_mode(inserted_inside):
+        bank = _bank(kind, g)
+    x, scores = _inputs(g, T)
+    with torch.inference_mode():
+        _near(moe_linear(x, scores, bank), x, scores, bank)
+    x.requires_grad_()
+    scores.requires_grad_()
+    y = moe_linear(x, scores, bank)
+    dx, ds = torch.autograd.grad(y, (x, scores), torch.ones_like(y))
+    assert dx.isfinite().all() and ds.isfinite().all() and dx.count_nonzero() > 0 and ds.count_nonzero() > 0
