@@ -51,7 +51,7 @@ class ExpertBank:
         self.experts: dict[int, object] = {}
         self._stack = None              # (ids, where their entries lie, stacked weight)
         self._streams = set()           # whose memory stacks are
-        self._fixed = False             # a captured graph reads the entries where they lie
+        self._fixed = False             # a captured graph reads the entries where they lie, or they do not fit twice
 
     def insert(self, expert_id: int, weight):
         """``weight``: a tensor (quantised on insertion) or an already quantised weight."""
@@ -90,8 +90,9 @@ class ExpertBank:
         that shape. The entries are moved into it (the same tensor objects on other memory), so that nothing is held twice and a
         change of an entry is a change of the stack. None where someone else holds an entry's memory (a caller's tensor, whose
         changes in place the bank has to follow), where an entry records gradients or was made in inference mode, where a captured
-        graph reads the entries (a call under capture moves nothing: the copies would only be recorded), or where the entries
-        are of different shapes, kinds or devices, or not stored as bf16, int4 or NF4."""
+        graph reads the entries (a call under capture moves nothing: the copies would only be recorded), where the device has
+        no room for a second copy meanwhile, or where the entries are of different shapes, kinds or devices, or not stored as
+        bf16, int4 or NF4."""
         with _MOVING:
             weight = self._stacked(tuple(ids))
         return None if weight is None else self._here(weight)
@@ -106,8 +107,12 @@ class ExpertBank:
         parts = _stackable(entries)
         if parts is None or not _sole_holders([t for part in parts for t in part]):
             return None
-        with torch.inference_mode(False), torch.no_grad():       # it outlives this call and its mode
-            joined = [torch.stack(part) for part in parts]
+        try:
+            with torch.inference_mode(False), torch.no_grad():       # it outlives this call and its mode
+                joined = [torch.stack(part) for part in parts]
+        except torch.OutOfMemoryError:
+            self._fixed = True
+            return None
         if joined[0].is_cuda:
             # every stream finds the stack filled, and nothing reads the old memory any more when it is given back
             torch.cuda.synchronize(joined[0].device)

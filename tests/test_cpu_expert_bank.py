@@ -183,3 +183,18 @@ def test_a_stack_made_in_inference_mode_is_an_ordinary_tensor():
     x = torch.ones(1, 64, dtype=BF, requires_grad=True)
     (x @ bank.stacked((0, 1))[0].t()).sum().backward()
     assert x.grad is not None
+
+
+def test_a_bank_that_does_not_fit_twice_stays_where_it_is(monkeypatch):
+    ws = _weights(2)
+    bank = ExpertBank("none")
+    for i, w in enumerate(ws):
+        bank.insert(i, w.clone())
+    tries = []
+
+    def full(tensors):
+        tries.append(tensors)
+        raise torch.OutOfMemoryError
+    monkeypatch.setattr(torch, "stack", full)
+    assert bank.stacked((0, 1)) is None and bank.stacked((0, 1)) is None and len(tries) == 1
+    assert all(torch.equal(bank.experts[i], w) for i, w in enumerate(ws))
