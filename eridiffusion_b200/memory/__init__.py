@@ -242,11 +242,19 @@ class QuantizedLinear(nn.Module):
         from ..ops import functional as F
         if self.adapter is not None:
             return self.adapter(self, x, act=act, residual=residual, gate=gate)
-        if F.on_codes(x, self.q):
+        shape = (*x.shape[:-1], self.out_features)
+        tokens = x.shape[-2] if x.dim() > 1 else 1
+        if x.numel() > 0 and F.on_codes(x, self.q) and self.weight_dtype == torch.bfloat16 and act in (None, "gelu", "silu") \
+                and F._native_ok(self.bias, residual, gate) and (residual is None or residual.shape == shape) \
+                and (gate is None or gate.shape == (x.numel() // (x.shape[-1] * tokens), self.out_features)):
             y = F.linear_4bit(x, self.q, bias=self.bias)
             if act is not None:
                 y = F.gelu_tanh(y) if act == "gelu" else F.silu(y)
-            return y if gate is None and residual is None else F.gate_residual(residual, y, gate)
+            if gate is None and residual is None:
+                return y
+            # a gate's row is that of the tokens in the last but one dimension
+            as_rows = (-1, tokens, self.out_features)
+            return F.gate_residual(None if residual is None else residual.reshape(as_rows), y.view(as_rows), gate).view(shape)
         return F.linear(x, self.weight, self.bias, act=act, residual=residual, gate=gate)
 
 
