@@ -254,7 +254,7 @@ Tensor expert_linear(const Tensor& x, const Tensor& w, const Tensor& offsets_, i
   return ExpertLinear::forward(nullptr, x, w, offsets, columns, accum);
 }
 
-// Nothing where the codes are not laid out for the kernel.
+// Nothing where the codes are not laid out for the kernel, or were made in inference mode and a gradient is asked for.
 OptT linear_4bit(const Tensor& x, const Tensor& codes, const Tensor& scale_, const OptT& offsets_, const OptT& bias_, int64_t experts,
                  int64_t N, int64_t block, bool nf4) {
   const Tensor bias = contig(opt(bias_));
@@ -268,8 +268,10 @@ OptT linear_4bit(const Tensor& x, const Tensor& codes, const Tensor& scale_, con
   const Tensor scale = contig(scale_.scalar_type() == at::kFloat ? scale_ : scale_.to(at::kFloat));
   const int64_t K = x.size(-1);
   const Tensor x2 = x.dim() == 2 ? x : x.reshape({-1, K});
-  Tensor y = any_grad({&x2, &bias}) ? Linear4bit::apply(x2, codes, scale, wrap(offsets), wrap(bias), experts, N, block, nf4)
-                                    : Linear4bit::forward(nullptr, x2, codes, scale, wrap(offsets), wrap(bias), experts, N, block, nf4);
+  const bool grad = any_grad({&x2, &bias});
+  if (grad && (codes.is_inference() || scale.is_inference())) return OptT();       // they cannot be kept for the backward pass
+  Tensor y = grad ? Linear4bit::apply(x2, codes, scale, wrap(offsets), wrap(bias), experts, N, block, nf4)
+                  : Linear4bit::forward(nullptr, x2, codes, scale, wrap(offsets), wrap(bias), experts, N, block, nf4);
   if (x.dim() == 2) return y;
   auto shape = x.sizes().vec();
   shape.back() = N;

@@ -79,3 +79,15 @@ def test_what_the_codes_do_not_take_goes_the_usual_way():
     with pytest.raises(RuntimeError):
         double(x)                                # types that do not go together, as before
     assert q(x[:, :0]).shape == (1, 0, 320)
+
+
+@pytest.mark.parametrize("kind", ["int4", "nf4"])
+def test_trained_after_quantising_in_inference_mode(kind):
+    g = torch.Generator(device="cuda").manual_seed(7)
+    with torch.inference_mode():
+        q = _layer(g, 320, 256, kind)
+    q.bias = None
+    x, dy = _mk(g, 3, 256).requires_grad_(), _mk(g, 3, 320)
+    (dx,) = torch.autograd.grad(q(x), x, dy)
+    w = q.q.dequantize(torch.float32).double()
+    assert ((dx.double() - dy.double() @ w).norm() / (dy.double() @ w).norm()).item() < 2 ** -7
