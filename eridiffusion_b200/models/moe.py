@@ -20,6 +20,7 @@ import sys
 import threading
 
 import torch
+from torch.autograd import forward_ad
 
 from ..memory import QuantizedTensor, dequantize, quantize
 from ..ops import functional as F
@@ -177,10 +178,18 @@ def select_topk_global(scores_or_total, k: int):
     return torch.topk(s, min(k, s.numel())).indices.tolist()
 
 
+def _plain(*ts) -> bool:
+    """Whether the kernels take these tensors: no forward-mode tangents, no transform (vmap, jvp, ..) and no subclass, for
+    which only PyTorch's own operations have rules."""
+    if torch._C._are_functorch_transforms_active() or any(type(t) not in (torch.Tensor, torch.nn.Parameter) for t in ts):
+        return False
+    return forward_ad._current_level < 0 or all(forward_ad.unpack_dual(t).tangent is None for t in ts)
+
+
 def route_tokens(scores: torch.Tensor, k: int, allowed=None):
     """Per-token top-k routing: returns (expert ids [tokens, k], normalised weights [tokens, k]).
     ``allowed``: restrict the choice to these expert ids (the resident set)."""
-    if scores.is_cuda and scores.dim() == 2 and F.get_backend() == "fused":
+    if scores.is_cuda and scores.dim() == 2 and F.get_backend() == "fused" and _plain(scores):
         mask = None
         if allowed is not None:
             mask = torch.zeros(scores.shape[1], dtype=torch.bool)
@@ -217,7 +226,7 @@ def moe_linear(x: torch.Tensor, scores: torch.Tensor, bank: ExpertBank, k: int =
 
 def _moe_grouped(x, idx, w, total: int, bank: ExpertBank, resident):
     """``moe_linear`` as one grouped product on the GPU; None where that does not apply."""
-    if not (x.is_cuda and x.dtype == torch.bfloat16 and x.dim() == 2 and x.shape[0] > 0 and F.get_backend() == "fused"):
+    if not (x.is_cuda and x.dtype == torch.bfloat16 and x.dim() == 2 and x.shape[0] > 0 and F.get_backend() == "fused" and _plain(x, w)):
         return None
     ids = [i for i in range(total) if i in bank.experts]
     if not ids:

@@ -3,7 +3,7 @@ import pytest
 import torch
 
 from eridiffusion_b200.memory import QuantizedTensor
-from eridiffusion_b200.models.moe import ExpertBank, moe_linear
+from eridiffusion_b200.models.moe import ExpertBank, moe_linear, route_tokens
 
 pytestmark = pytest.mark.gpu
 BF = torch.bfloat16
@@ -183,3 +183,43 @@ def test_training_after_a_call_in_inference_mode(kind, inserted_inside, T):
     y = moe_linear(x, scores, bank)
     dx, ds = torch.autograd.grad(y, (x, scores), torch.ones_like(y))
     assert dx.isfinite().all() and ds.isfinite().all() and dx.count_nonzero() > 0 and ds.count_nonzero() > 0
+
+
+def _far_apart(g, T):
+    """Scores whose order no small step changes."""
+    return torch.stack([torch.randperm(E, device="cuda", generator=g) for _ in range(T)]).float()
+
+
+@pytest.mark.parametrize("dual", ["x", "scores"])
+def test_forward_mode(dual):
+    g = torch.Generator(device="cuda").manual_seed(11)
+    bank = _bank("none", g)
+    x, scores = _mk(g, 7, K), _far_apart(g, 7)
+    tangent = torch.randn(7, K if dual == "x" else E, device="cuda", generator=g)
+    with torch.autograd.forward_ad.dual_level():
+        if dual == "x":
+            y = moe_linear(torch.autograd.forward_ad.make_dual(x, tangent.to(BF)), scores, bank)
+        else:
+            y = moe_linear(x, torch.autograd.forward_ad.make_dual(scores, tangent), bank)
+        out = torch.autograd.forward_ad.unpack_dual(y)
+    top, idx = torch.sort(scores.double(), dim=-1, descending=True)
+    w = torch.softmax(top[:, :2], -1)
+    experts = torch.stack([bank.experts[e].double() for e in range(E)])[idx[:, :2]]                # [T, 2, N, K]
+    if dual == "x":
+        ref = (w[..., None] * torch.einsum("tjnk,tk->tjn", experts, tangent.to(BF).double())).sum(1)
+    else:
+        dtop = tangent.double().gather(1, idx[:, :2])
+        dw = w * (dtop - (w * dtop).sum(-1, keepdim=True))
+        ref = (dw[..., None] * torch.einsum("tjnk,tk->tjn", experts, x.double())).sum(1)
+    assert out.tangent is not None and ((out.tangent.double() - ref).norm() / ref.norm()).item() < 2 ** -6
+
+
+def test_router_under_transforms():
+    g = torch.Generator(device="cuda").manual_seed(12)
+    s = torch.stack([_far_apart(g, 5) for _ in range(3)])
+    idx, w = torch.func.vmap(lambda t: route_tokens(t, 2))(s)
+    for b in range(3):
+        i1, w1 = route_tokens(s[b], 2)
+        assert torch.equal(idx[b], i1) and torch.allclose(w[b], w1, atol=1e-6)
+    _, dw = torch.func.jvp(lambda t: route_tokens(t, 2)[1], (s[0],), (torch.ones_like(s[0]),))
+    assert dw.abs().max().item() < 1e-6           # weights do not change when all scores grow alike
