@@ -1,9 +1,12 @@
 // Token-routed experts and products on 4-bit weights as autograd nodes: router, plan, dispatch, combine, the product grouped by
 // expert and the product on codes. Shapes, types and devices are checked by ops/functional.py; nothing here reads a value back
-// from the device.
+// from the device. A backward pass that is recorded itself (create_graph) runs on nodes and operations that have gradients; operands are
+// laid out before a node takes them, so that what it saves is what autograd knows.
 #include "eri_ops.h"
 
 #include <c10/cuda/CUDAGuard.h>
+
+#include <limits>
 
 namespace eri_ops {
 
@@ -20,14 +23,26 @@ Rows rows_of(const Tensor& t) {
   if (rows_ok(t) && t.stride(0) >= t.size(1)) return {t, (long long)t.stride(0)};
   return {contig16(t), (long long)t.size(1)};
 }
+bool recorded() { return at::GradMode::is_enabled(); }       // inside a backward pass
 const int* ints(const Tensor& t) { return t.defined() ? (const int*)t.data_ptr() : nullptr; }
 
 // ------------------------------------------------------------------------------------------- router
 struct ExpertRoute : torch::autograd::Function<ExpertRoute> {
-  static variable_list forward(AutogradContext* ctx, const Tensor& scores, const OptT& allowed_o, int64_t k, bool normalize) {
+  // The backward kernel's formulas (a row that may choose nothing has weights and gradients of zero).
+  static Tensor gradient(const Tensor& s, const Tensor& allowed, const Tensor& idx, const Tensor& dw, bool normalize) {
+    Tensor f = s.to(at::kFloat);
+    if (allowed.defined()) f = f.masked_fill(allowed.logical_not(), -std::numeric_limits<float>::infinity());
+    const Tensor top = f.gather(1, idx), first = top.detach().narrow(1, 0, 1);
+    const Tensor m = first.masked_fill(first == -std::numeric_limits<float>::infinity(), 0.f);
+    const Tensor z = (top - m).exp(), all = normalize ? z : (f - m).exp(), sum = all.sum(1, true), total = sum.masked_fill(sum == 0, 1.f);
+    const Tensor w = z / total, dot = (w * dw).sum(1, true), none = at::zeros(s.sizes(), f.options());
+    Tensor ds = normalize ? none.scatter(1, idx, w * (dw - dot)) : all / total * (none.scatter(1, idx, dw) - dot);
+    if (allowed.defined()) ds = ds.masked_fill(allowed.logical_not(), 0.f);
+    return ds.to(s.scalar_type());
+  }
+  static variable_list forward(AutogradContext* ctx, const Tensor& s, const OptT& allowed_o, int64_t k, bool normalize) {
     const Tensor allowed = opt(allowed_o);
-    const CUDAGuard guard(scores.device());
-    const Tensor s = scores.stride(1) == 1 && scores.stride(0) >= scores.size(1) ? scores : scores.contiguous();
+    const CUDAGuard guard(s.device());
     const int64_t T = s.size(0), E = s.size(1);
     const long long ld = s.is_contiguous() ? E : s.stride(0);
     Tensor idx = at::empty({T, k}, s.options().dtype(at::kLong)), w = empty_f32({T, k}, s);
@@ -48,6 +63,10 @@ struct ExpertRoute : torch::autograd::Function<ExpertRoute> {
     const Tensor &s = sv[0], &allowed = sv[1], &idx = sv[2], &w = sv[3];
     const auto m = ctx->saved_data["m"].toIntVector();
     const CUDAGuard guard(s.device());
+    if (recorded()) {
+      out[0] = gradient(s, allowed, idx, gout[1], m[1]);
+      return out;
+    }
     const Tensor dw = contig(gout[1]);
     Tensor ds = at::empty({s.size(0), s.size(1)}, s.options());
     check(L.eri_expert_route_bwd(s.data_ptr(), m[2], ptr(allowed), idx.data_ptr(), (const float*)w.data_ptr(),
@@ -79,20 +98,30 @@ Tensor gather(const Tensor& y_, const Tensor& rows, const Tensor& w) {
 struct ExpertDispatch : torch::autograd::Function<ExpertDispatch> {
   static Tensor forward(AutogradContext* ctx, const Tensor& x, const Tensor& rows, const Tensor& offsets) {
     const CUDAGuard guard(x.device());
-    if (ctx) ctx->save_for_backward({rows});
+    if (ctx) ctx->save_for_backward({rows, offsets});
     return scatter(x, rows, offsets);
   }
   static variable_list backward(AutogradContext* ctx, variable_list gout) {
-    const Tensor rows = ctx->get_saved_variables()[0];
+    auto sv = ctx->get_saved_variables();
+    const Tensor &rows = sv[0], &offsets = sv[1];
     const CUDAGuard guard(rows.device());
+    if (recorded()) return {expert_combine(gout[0], at::ones(rows.sizes(), rows.options().dtype(at::kFloat)), rows, offsets), Tensor(), Tensor()};
     return {gather(gout[0], rows, Tensor()), Tensor(), Tensor()};
   }
 };
 
 struct ExpertCombine : torch::autograd::Function<ExpertCombine> {
-  static Tensor forward(AutogradContext* ctx, const Tensor& y, const Tensor& w_, const Tensor& rows, const Tensor& offsets) {
+  // dy and dw in operations that have gradients; choices of nobody go to a row of their own behind the others.
+  static std::pair<Tensor, Tensor> gradient(const Tensor& dout, const Tensor& y, const Tensor& w, const Tensor& rows) {
+    const int64_t T = rows.size(0), k = rows.size(1), D = y.size(1);
+    const Tensor nobody = (rows < 0).unsqueeze(-1), d = dout.to(at::kFloat).unsqueeze(1);
+    const Tensor yt = y.index_select(0, rows.clamp_min(0).flatten()).view({T, k, D}).to(at::kFloat).masked_fill(nobody, 0.f);
+    const Tensor dw = (d * yt).sum(-1), dyt = (w.unsqueeze(-1) * d).to(y.scalar_type()).reshape({T * k, D});
+    const Tensor to = rows.masked_fill(rows < 0, T * k).flatten().to(at::kLong);
+    return {at::zeros({T * k + 1, D}, y.options()).index_copy(0, to, dyt).narrow(0, 0, T * k), dw};
+  }
+  static Tensor forward(AutogradContext* ctx, const Tensor& y, const Tensor& w, const Tensor& rows, const Tensor& offsets) {
     const CUDAGuard guard(y.device());
-    const Tensor w = contig(w_);
     if (ctx) ctx->save_for_backward({y, w, rows, offsets});
     return gather(y, rows, w);
   }
@@ -100,6 +129,10 @@ struct ExpertCombine : torch::autograd::Function<ExpertCombine> {
     auto sv = ctx->get_saved_variables();
     const Tensor &w = sv[1], &rows = sv[2], &offsets = sv[3];
     const CUDAGuard guard(rows.device());
+    if (recorded()) {
+      const auto [gy, gw] = gradient(gout[0], sv[0], w, rows);
+      return {ctx->needs_input_grad(0) ? gy : Tensor(), ctx->needs_input_grad(1) ? gw : Tensor(), Tensor(), Tensor()};
+    }
     const Rows y = rows_of(sv[0]), d = rows_of(gout[0]);
     const int64_t T = rows.size(0), k = rows.size(1), D = y.t.size(1), E = offsets.size(0) - 1;
     Tensor dy, dw;
@@ -115,44 +148,74 @@ struct ExpertCombine : torch::autograd::Function<ExpertCombine> {
 // ------------------------------------------------------------------------------------------- grouped product
 enum { kFwd = 0, kDx = 1, kDw = 2 };
 
+// dw[e] = dy^T x over the rows of expert e, in `out` or added to it.
+void weight_gradient(const Tensor& x_, const Tensor& dy_, const Tensor& offsets, const Tensor& out, bool accum) {
+  const Rows x = rows_of(x_), dy = rows_of(dy_);
+  const int64_t R = x.t.size(0), E = out.size(0), N = out.size(1), K = out.size(2);
+  if (R > 0)
+    check(L.eri_expert_gemm(kDw, x.t.data_ptr(), x.ld, dy.t.data_ptr(), dy.ld, nullptr, ints(offsets), out.data_ptr(), (int)R, (int)E, (int)N,
+                            (int)K, 0, accum, extent(out), stream()), "expert_gemm_dw");
+  else if (!accum)
+    out.zero_();
+}
+// The same as a node, for backward passes that are recorded.
+struct ExpertWeightGradient : torch::autograd::Function<ExpertWeightGradient> {
+  static Tensor forward(AutogradContext* ctx, const Tensor& x, const Tensor& dy, const Tensor& offsets) {
+    const CUDAGuard guard(x.device());
+    ctx->save_for_backward({x, dy, offsets});
+    Tensor out = empty_bf16({offsets.size(0) - 1, dy.size(1), x.size(1)}, x);
+    weight_gradient(x, dy, offsets, out, false);
+    return out;
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list gout) {
+    auto sv = ctx->get_saved_variables();
+    const Tensor &x = sv[0], &dy = sv[1], &offsets = sv[2];
+    Tensor gx, gdy;
+    if (ctx->needs_input_grad(0)) gx = expert_linear(dy, gout[0].transpose(1, 2), offsets, 0, false);
+    if (ctx->needs_input_grad(1)) gdy = expert_linear(x, gout[0], offsets, 0, false);
+    return {gx, gdy, Tensor()};
+  }
+};
+
 struct ExpertLinear : torch::autograd::Function<ExpertLinear> {
-  static Tensor forward(AutogradContext* ctx, const Tensor& x_, const Tensor& w_, const Tensor& offsets, int64_t columns, bool accum) {
+  static Tensor forward(AutogradContext* ctx, const Tensor& x_, const Tensor& w, const Tensor& offsets, int64_t columns, bool accum) {
     const CUDAGuard guard(x_.device());
     const Rows x = rows_of(x_);
-    const Tensor w = contig16(w_);
     const int64_t R = x.t.size(0), E = w.size(0), N = w.size(1), K = w.size(2);
     Tensor y = empty_bf16({R, N}, x.t);
     if (R > 0)
       check(L.eri_expert_gemm(kFwd, x.t.data_ptr(), x.ld, nullptr, 0, w.data_ptr(), ints(offsets), y.data_ptr(), (int)R, (int)E, (int)N,
                               (int)K, (int)columns, 0, extent(y), stream()), "expert_gemm");
     if (ctx) {
-      ctx->save_for_backward({x.t, w, offsets, w_});
-      ctx->saved_data["m"] = std::vector<int64_t>{x.ld, columns, accum};
+      ctx->save_for_backward({x_, w, offsets});
+      ctx->saved_data["m"] = std::vector<int64_t>{columns, accum};
     }
     return y;
   }
   static variable_list backward(AutogradContext* ctx, variable_list gout) {
     auto sv = ctx->get_saved_variables();
-    const Tensor &x = sv[0], &w = sv[1], &offsets = sv[2], &param = sv[3];
+    const Tensor &x = sv[0], &w = sv[1], &offsets = sv[2];
     const auto m = ctx->saved_data["m"].toIntVector();
-    const CUDAGuard guard(x.device());
-    const Rows dy = rows_of(gout[0]);
-    const int64_t R = x.size(0), E = w.size(0), N = w.size(1), K = w.size(2);
+    const CUDAGuard guard(w.device());
+    const int64_t E = w.size(0), N = w.size(1), K = w.size(2);
     Tensor dx, dw;
+    if (recorded()) {
+      if (ctx->needs_input_grad(0)) dx = expert_linear(gout[0], w.transpose(1, 2), offsets, m[0], false);
+      if (ctx->needs_input_grad(1)) dw = ExpertWeightGradient::apply(x, gout[0], offsets);
+      return {dx, dw, Tensor(), Tensor(), Tensor()};
+    }
+    const Rows dy = rows_of(gout[0]);
     if (ctx->needs_input_grad(0)) {
-      dx = empty_bf16({R, K}, x);
+      const int64_t R = dy.t.size(0);
+      dx = empty_bf16({R, K}, dy.t);
       if (R > 0)
         check(L.eri_expert_gemm(kDx, dy.t.data_ptr(), dy.ld, nullptr, 0, w.data_ptr(), ints(offsets), dx.data_ptr(), (int)R, (int)E,
-                                (int)N, (int)K, (int)m[1], 0, extent(dx), stream()), "expert_gemm_dx");
+                                (int)N, (int)K, (int)m[0], 0, extent(dx), stream()), "expert_gemm_dx");
     }
     if (ctx->needs_input_grad(1)) {
-      const bool acc = has_grad_buffer(param, at::kBFloat16, m[2]) && al16(param.grad());
-      Tensor out = acc ? param.grad() : empty_bf16({E, N, K}, x);
-      if (R > 0)
-        check(L.eri_expert_gemm(kDw, x.data_ptr(), m[0], dy.t.data_ptr(), dy.ld, nullptr, ints(offsets), out.data_ptr(), (int)R, (int)E,
-                                (int)N, (int)K, 0, acc, extent(out), stream()), "expert_gemm_dw");
-      else if (!acc)
-        out.zero_();
+      const bool acc = has_grad_buffer(w, at::kBFloat16, m[1]) && al16(w.grad());
+      Tensor out = acc ? w.grad() : empty_bf16({E, N, K}, w);
+      weight_gradient(x, dy.t, offsets, out, acc);
       if (!acc) dw = out;
     }
     return {dx, dw, Tensor(), Tensor(), Tensor()};
@@ -160,6 +223,36 @@ struct ExpertLinear : torch::autograd::Function<ExpertLinear> {
 };
 
 // ------------------------------------------------------------------------------------------- 4-bit codes
+// dx = dy W on the codes.
+Tensor codes_gradient(const Tensor& dy_, const Tensor& codes, const Tensor& scale, const Tensor& offsets, int E, int N, int K, int block, bool nf4) {
+  const CUDAGuard guard(codes.device());
+  const Tensor dy = contig16(dy_);
+  const int R = (int)dy.size(0);
+  Tensor dx = empty_bf16({R, K}, dy);
+  if (R > 0) {
+    Tensor work = empty_f32({L.eri_linear_4bit_planes(R, N, K, block, offsets.defined()), R, K}, dy);
+    check(L.eri_linear_4bit_dgrad(dy.data_ptr(), N, codes.data_ptr(), (const float*)scale.data_ptr(), ints(offsets), (float*)work.data_ptr(),
+                                  dx.data_ptr(), R, E, N, K, block, nf4, stream()), "linear_4bit_dgrad");
+  }
+  return dx;
+}
+// The same as a node, for backward passes that are recorded.
+struct Linear4bitGradient : torch::autograd::Function<Linear4bitGradient> {
+  static Tensor forward(AutogradContext* ctx, const Tensor& dy, const Tensor& codes, const Tensor& scale, const OptT& offsets_o, int64_t E,
+                        int64_t N, int64_t K, int64_t block, bool nf4) {
+    ctx->save_for_backward({codes, scale, opt(offsets_o)});
+    ctx->saved_data["m"] = std::vector<int64_t>{E, N, block, nf4};
+    return codes_gradient(dy, codes, scale, opt(offsets_o), (int)E, (int)N, (int)K, (int)block, nf4);
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list gout) {
+    auto sv = ctx->get_saved_variables();
+    const auto m = ctx->saved_data["m"].toIntVector();
+    variable_list out(9);
+    out[0] = *linear_4bit(gout[0], sv[0], sv[1], wrap(sv[2]), OptT(), m[0], m[1], m[2], m[3]);
+    return out;
+  }
+};
+
 struct Linear4bit : torch::autograd::Function<Linear4bit> {
   static Tensor forward(AutogradContext* ctx, const Tensor& x_, const Tensor& codes, const Tensor& scale, const OptT& offsets_o,
                         const OptT& bias_o, int64_t E, int64_t N, int64_t block, bool nf4) {
@@ -181,19 +274,11 @@ struct Linear4bit : torch::autograd::Function<Linear4bit> {
     auto sv = ctx->get_saved_variables();
     const Tensor &codes = sv[0], &scale = sv[1], &offsets = sv[2];
     const auto m = ctx->saved_data["m"].toIntVector();
-    const int R = (int)m[0], K = (int)m[1], E = (int)m[2], N = (int)m[3];
     const CUDAGuard guard(codes.device());
     Tensor dx, db;
-    if (ctx->needs_input_grad(0)) {
-      const Tensor dy = contig16(gout[0]);
-      dx = empty_bf16({R, K}, dy);
-      if (R > 0) {
-        Tensor work = empty_f32({L.eri_linear_4bit_planes(R, N, K, (int)m[4], offsets.defined()), R, K}, dy);
-        check(L.eri_linear_4bit_dgrad(dy.data_ptr(), N, codes.data_ptr(), (const float*)scale.data_ptr(), ints(offsets),
-                                      (float*)work.data_ptr(), dx.data_ptr(), R, E, N, K, (int)m[4], (int)m[5], stream()),
-              "linear_4bit_dgrad");
-      }
-    }
+    if (ctx->needs_input_grad(0))
+      dx = recorded() ? Linear4bitGradient::apply(gout[0], codes, scale, wrap(offsets), m[2], m[3], m[1], m[4], (bool)m[5])
+                      : codes_gradient(gout[0], codes, scale, offsets, (int)m[2], (int)m[3], (int)m[1], (int)m[4], m[5]);
     // an absent optional argument has no edge; a bias comes without offsets
     if (m[6] && ctx->needs_input_grad(3)) db = gout[0].sum(0);
     return {dx, Tensor(), Tensor(), Tensor(), db, Tensor(), Tensor(), Tensor(), Tensor()};
@@ -217,8 +302,10 @@ Tensor int32(const Tensor& t) { return contig(t.scalar_type() == at::kInt ? t : 
 std::vector<Tensor> expert_route(const Tensor& scores, const OptT& allowed_, int64_t k, bool normalize) {
   const Tensor allowed = contig(opt(allowed_));
   same_device("expert_route", scores, {&allowed});
-  if (any_grad({&scores})) return ExpertRoute::apply(scores, wrap(allowed), k, normalize);
-  return ExpertRoute::forward(nullptr, scores, wrap(allowed), k, normalize);
+  const bool grad = any_grad({&scores});
+  const Tensor s = scores.stride(1) == 1 && scores.stride(0) >= scores.size(1) ? scores : scores.contiguous();
+  if (grad) return ExpertRoute::apply(s, wrap(allowed), k, normalize);
+  return ExpertRoute::forward(nullptr, s, wrap(allowed), k, normalize);
 }
 
 std::vector<Tensor> expert_plan(const Tensor& idx_, int64_t experts) {
@@ -239,18 +326,20 @@ Tensor expert_dispatch(const Tensor& x, const Tensor& rows, const Tensor& offset
   return ExpertDispatch::forward(nullptr, x, rows, offsets);
 }
 
-Tensor expert_combine(const Tensor& y, const Tensor& w_, const Tensor& rows, const Tensor& offsets) {
-  same_device("expert_combine", y, {&w_, &rows, &offsets});
+Tensor expert_combine(const Tensor& y_, const Tensor& w_, const Tensor& rows, const Tensor& offsets) {
+  same_device("expert_combine", y_, {&w_, &rows, &offsets});
   check_plan("expert_combine", rows, offsets);
-  const Tensor w = w_.scalar_type() == at::kFloat ? w_ : w_.to(at::kFloat);
-  if (any_grad({&y, &w})) return ExpertCombine::apply(y, w, rows, offsets);
+  const bool grad = any_grad({&y_, &w_});
+  const Tensor y = rows_of(y_).t, w = contig(w_.scalar_type() == at::kFloat ? w_ : w_.to(at::kFloat));
+  if (grad) return ExpertCombine::apply(y, w, rows, offsets);
   return ExpertCombine::forward(nullptr, y, w, rows, offsets);
 }
 
-Tensor expert_linear(const Tensor& x, const Tensor& w, const Tensor& offsets_, int64_t columns, bool accum) {
-  same_device("expert_linear", x, {&w, &offsets_});
-  const Tensor offsets = int32(offsets_);
-  if (any_grad({&x, &w})) return ExpertLinear::apply(x, w, offsets, columns, accum);
+Tensor expert_linear(const Tensor& x_, const Tensor& w_, const Tensor& offsets_, int64_t columns, bool accum) {
+  same_device("expert_linear", x_, {&w_, &offsets_});
+  const bool grad = any_grad({&x_, &w_});
+  const Tensor offsets = int32(offsets_), x = rows_of(x_).t, w = contig16(w_);
+  if (grad) return ExpertLinear::apply(x, w, offsets, columns, accum);
   return ExpertLinear::forward(nullptr, x, w, offsets, columns, accum);
 }
 
