@@ -112,32 +112,33 @@ struct ExpertDispatch : torch::autograd::Function<ExpertDispatch> {
 
 struct ExpertCombine : torch::autograd::Function<ExpertCombine> {
   // dy and dw in operations that have gradients; choices of nobody go to a row of their own behind the others.
-  static std::pair<Tensor, Tensor> gradient(const Tensor& dout, const Tensor& y, const Tensor& w, const Tensor& rows) {
-    const int64_t T = rows.size(0), k = rows.size(1), D = y.size(1);
-    const Tensor nobody = (rows < 0).unsqueeze(-1), d = dout.to(at::kFloat).unsqueeze(1);
-    const Tensor yt = y.index_select(0, rows.clamp_min(0).flatten()).view({T, k, D}).to(at::kFloat).masked_fill(nobody, 0.f);
-    const Tensor dw = (d * yt).sum(-1), dyt = (w.unsqueeze(-1) * d).to(y.scalar_type()).reshape({T * k, D});
-    const Tensor to = rows.masked_fill(rows < 0, T * k).flatten().to(at::kLong);
-    return {at::zeros({T * k + 1, D}, y.options()).index_copy(0, to, dyt).narrow(0, 0, T * k), dw};
+  static Tensor gradient_rows(const Tensor& dout, const Tensor& w, const Tensor& rows) {
+    const int64_t n = rows.numel(), D = dout.size(1);
+    const Tensor dy = (w.unsqueeze(-1) * dout.to(at::kFloat).unsqueeze(1)).to(dout.scalar_type()).reshape({n, D});
+    const Tensor to = rows.masked_fill(rows < 0, n).flatten().to(at::kLong);
+    return at::zeros({n + 1, D}, dout.options()).index_copy(0, to, dy).narrow(0, 0, n);
+  }
+  static Tensor gradient_weights(const Tensor& dout, const Tensor& y, const Tensor& rows) {
+    const Tensor yt = y.index_select(0, rows.clamp_min(0).flatten()).view({rows.size(0), rows.size(1), y.size(1)}).to(at::kFloat);
+    return (dout.to(at::kFloat).unsqueeze(1) * yt.masked_fill((rows < 0).unsqueeze(-1), 0.f)).sum(-1);
   }
   static Tensor forward(AutogradContext* ctx, const Tensor& y, const Tensor& w, const Tensor& rows, const Tensor& offsets) {
     const CUDAGuard guard(y.device());
-    if (ctx) ctx->save_for_backward({y, w, rows, offsets});
+    if (ctx) ctx->save_for_backward({w.requires_grad() ? y : Tensor(), w, rows, offsets});
     return gather(y, rows, w);
   }
   static variable_list backward(AutogradContext* ctx, variable_list gout) {
     auto sv = ctx->get_saved_variables();
     const Tensor &w = sv[1], &rows = sv[2], &offsets = sv[3];
     const CUDAGuard guard(rows.device());
-    if (recorded()) {
-      const auto [gy, gw] = gradient(gout[0], sv[0], w, rows);
-      return {ctx->needs_input_grad(0) ? gy : Tensor(), ctx->needs_input_grad(1) ? gw : Tensor(), Tensor(), Tensor()};
-    }
-    const Rows y = rows_of(sv[0]), d = rows_of(gout[0]);
-    const int64_t T = rows.size(0), k = rows.size(1), D = y.t.size(1), E = offsets.size(0) - 1;
+    if (recorded())
+      return {ctx->needs_input_grad(0) ? gradient_rows(gout[0], w, rows) : Tensor(),
+              ctx->needs_input_grad(1) ? gradient_weights(gout[0], sv[0], rows) : Tensor(), Tensor(), Tensor()};
+    const Rows d = rows_of(gout[0]), y = ctx->needs_input_grad(1) ? rows_of(sv[0]) : d;       // y: for dw alone
+    const int64_t T = rows.size(0), k = rows.size(1), D = d.t.size(1), E = offsets.size(0) - 1;
     Tensor dy, dw;
-    if (ctx->needs_input_grad(0)) dy = empty_bf16({T * k, D}, y.t);
-    if (ctx->needs_input_grad(1)) dw = empty_f32({T, k}, y.t);
+    if (ctx->needs_input_grad(0)) dy = empty_bf16({T * k, D}, d.t);
+    if (ctx->needs_input_grad(1)) dw = empty_f32({T, k}, d.t);
     if (dy.defined() || dw.defined())
       check(L.eri_expert_gather_bwd(d.t.data_ptr(), d.ld, y.t.data_ptr(), y.ld, ints(rows), (const float*)w.data_ptr(), ints(offsets) + E,
                                     mptr(dy), (float*)mptr(dw), (int)T, (int)k, (int)(T * k), (int)D, stream()), "expert_gather_bwd");
@@ -162,7 +163,7 @@ void weight_gradient(const Tensor& x_, const Tensor& dy_, const Tensor& offsets,
 struct ExpertWeightGradient : torch::autograd::Function<ExpertWeightGradient> {
   static Tensor forward(AutogradContext* ctx, const Tensor& x, const Tensor& dy, const Tensor& offsets) {
     const CUDAGuard guard(x.device());
-    ctx->save_for_backward({x, dy, offsets});
+    ctx->save_for_backward({dy.requires_grad() ? x : Tensor(), x.requires_grad() ? dy : Tensor(), offsets});
     Tensor out = empty_bf16({offsets.size(0) - 1, dy.size(1), x.size(1)}, x);
     weight_gradient(x, dy, offsets, out, false);
     return out;
@@ -187,7 +188,7 @@ struct ExpertLinear : torch::autograd::Function<ExpertLinear> {
       check(L.eri_expert_gemm(kFwd, x.t.data_ptr(), x.ld, nullptr, 0, w.data_ptr(), ints(offsets), y.data_ptr(), (int)R, (int)E, (int)N,
                               (int)K, (int)columns, 0, extent(y), stream()), "expert_gemm");
     if (ctx) {
-      ctx->save_for_backward({x_, w, offsets});
+      ctx->save_for_backward({w.requires_grad() ? x_ : Tensor(), w, offsets});       // a frozen weight leaves nothing to do with x
       ctx->saved_data["m"] = std::vector<int64_t>{columns, accum};
     }
     return y;

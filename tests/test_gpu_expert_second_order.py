@@ -139,3 +139,27 @@ def test_moe_linear(kind, T):
         w = torch.softmax(s.gather(1, idx), -1)
         return (w[..., None] * torch.einsum("tjnk,tk->tjn", ws[idx], x)).sum(1)
     _compare(lambda x, s: moe_linear(x, s, bank, k), ref, [_mk(g, T, K), scores], _mk(g, T, N), g, 8 * 2 ** -8)
+
+
+@pytest.mark.parametrize("trained", ["x", "w", "both"])
+def test_only_what_a_gradient_needs_is_kept(trained):
+    """A frozen weight keeps no tokens, a weight without gradient no expert outputs; the gradients are those of the full pass."""
+    g = torch.Generator(device="cuda").manual_seed(8)
+    T, k, E, D = 20, 2, 4, 64
+    plan = _plan(g, T, k, E)
+    x, w = _mk(g, T * k, D), _mk(g, E, 72, D, std=0.1)
+    y, f = _mk(g, T * k, D), torch.rand(T, k, device="cuda", generator=g)
+    dx, dout = _mk(g, T * k, 72), _mk(g, T, D)
+    full = [t.clone().requires_grad_() for t in (x, w, y, f)]
+    want = [*torch.autograd.grad(F.expert_linear(full[0], full[1], plan.offsets), full[:2], dx),
+            *torch.autograd.grad(F.expert_combine(full[2], full[3], plan), full[2:], dout)]
+    pick = {"x": (0,), "w": (1,), "both": (0, 1)}[trained]
+    for i in pick:
+        (x, w)[i].requires_grad_()
+        (y, f)[i].requires_grad_()
+    kept = []
+    with torch.autograd.graph.saved_tensors_hooks(lambda t: (kept.append(t.data_ptr()), t)[1], lambda t: t):
+        a, b = F.expert_linear(x, w, plan.offsets), F.expert_combine(y, f, plan)
+    assert (x.data_ptr() in kept) == (1 in pick) and (y.data_ptr() in kept) == (1 in pick)
+    got = [*torch.autograd.grad(a, [(x, w)[i] for i in pick], dx), *torch.autograd.grad(b, [(y, f)[i] for i in pick], dout)]
+    assert all(torch.equal(p, q) for p, q in zip(got, [want[i] for i in pick] + [want[2 + i] for i in pick]))
