@@ -7,6 +7,7 @@
 // e: the expert of row r, offsets[e] <= r < offsets[e + 1] (offsets null: one weight for all rows). Rows of no expert are zeros. Up to
 // eight rows of one expert share a pass over its codes.
 #include <cuda_fp16.h>
+#include <limits.h>
 
 #include "ptx.cuh"
 
@@ -25,19 +26,23 @@ __constant__ float c_nf4[16] = {-1.0f, -0.6961928009986877f, -0.5250730514526367
 struct Segment {
   int e, rows;        // rows of this CTA from row r on: 0 = another CTA's, -1 = row r belongs to no expert
 };
-// offsets ascend; whatever they hold, the rows stay in [0, R).
-__device__ __forceinline__ Segment segment_of(const int* offsets, int E, int R, int r, int most) {
+// The bounds are the running maximum of the offsets inside [0, R], whatever they hold (expert_table, too): row r belongs to the
+// expert before the first offset above r, from the largest offset before that one on. By a whole warp.
+__device__ __forceinline__ Segment segment_of(const int* offsets, int E, int R, int r, int most, int lane) {
   if (!offsets) return Segment{0, r % most == 0 ? min(most, R - r) : 0};
-  int lo = 0, hi = E + 1;                // the last e with offsets[e] <= r, plus one
-  while (lo < hi) {
-    const int mid = (lo + hi) >> 1;
-    if (offsets[mid] <= r) lo = mid + 1; else hi = mid;
+  int first = 0;
+  for (int e0 = 0; e0 <= E; e0 += 32) {
+    const int o = e0 + lane <= E ? offsets[e0 + lane] : INT_MIN;
+    const unsigned above = __ballot_sync(0xffffffffu, o > r);
+    const int at = above ? __ffs(above) - 1 : 32;
+    first = max(first, __reduce_max_sync(0xffffffffu, lane < at ? o : INT_MIN));
+    if (above) {
+      const int end = min(R, __shfl_sync(0xffffffffu, o, at)), e = e0 + at - 1;
+      if (e < 0) break;
+      return Segment{e, (r - first) % most == 0 ? min(most, end - r) : 0};
+    }
   }
-  const int e = lo - 1;
-  if (e < 0 || e >= E) return Segment{0, -1};
-  const int first = max(0, offsets[e]), end = min(R, offsets[e + 1]);
-  if (r < first || r >= end) return Segment{0, -1};
-  return Segment{e, (r - first) % most == 0 ? min(most, end - r) : 0};
+  return Segment{0, -1};
 }
 
 // ------------------------------------------------------------------------------------------- y = x W^T
@@ -477,9 +482,10 @@ __global__ void __launch_bounds__(kDgWarps * 32, 1) dgrad_4bit_kernel(const DgAr
   extern __shared__ __align__(16) uint8_t sm4[];
   __shared__ __align__(128) uint8_t table[NF4 ? kTable : 16];
   const int r0 = p.offsets ? (int)blockIdx.y : (int)blockIdx.y * kRows;
-  const Segment sg = segment_of(p.offsets, p.E, p.R, r0, kRows);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const Segment sg = segment_of(p.offsets, p.E, p.R, r0, kRows, lane);
   if (sg.rows == 0) return;
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+  const int g = lane >> 2, t = lane & 3;
   const int k0 = blockIdx.x * kCols;
   const int M = sg.rows < 0 ? 1 : sg.rows, steps = p.K / STEP;
   float* plane = p.part + ((long long)blockIdx.z * p.R + r0) * p.K;
