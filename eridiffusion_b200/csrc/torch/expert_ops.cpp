@@ -297,7 +297,8 @@ void check_plan(const char* what, const Tensor& rows, const Tensor& offsets) {
   TORCH_CHECK_VALUE(rows.scalar_type() == at::kInt && rows.is_contiguous() && offsets.scalar_type() == at::kInt && offsets.is_contiguous() &&
                         offsets.dim() == 1 && offsets.size(0) > 1, what, ": not a plan of expert_plan");
 }
-Tensor int32(const Tensor& t) { return contig(t.scalar_type() == at::kInt ? t : t.to(at::kInt)); }
+// Offsets as the kernels take them; rows are fewer than 2^31, so a wider offset is one behind them all.
+Tensor int32(const Tensor& t) { return contig(t.scalar_type() == at::kInt ? t : t.clamp(0, std::numeric_limits<int>::max()).to(at::kInt)); }
 }  // namespace
 
 std::vector<Tensor> expert_route(const Tensor& scores, const OptT& allowed_, int64_t k, bool normalize) {

@@ -59,3 +59,16 @@ def test_same_rows_in_both_directions(name, dtype):
         if q is None:
             _check(grads[1], torch.einsum("re,rn,rk->enk", pick, dd, xd), torch.einsum("re,rn,rk->enk", pick, dd.abs(), xd.abs()), rows)
     assert F.kernel_error_check() == {}
+
+
+def test_offsets_wider_than_32_bits():
+    g = torch.Generator(device="cuda").manual_seed(1)
+    x, w = _mk(g, 10, 128), _mk(g, 2, 88, 128)
+    q = quantize(w, "nf4")
+    wide = torch.tensor([0, 4, 2 ** 32 + 1], device="cuda")              # the low 32 bits are 1
+    near = torch.tensor([-2 ** 32 + 9, 4, 10], device="cuda")
+    want = torch.tensor([0, 4, 10], dtype=torch.int32, device="cuda")
+    for off in (wide, near):
+        assert torch.equal(F.expert_linear(x, w, off), F.expert_linear(x, w, want))
+        assert torch.equal(F.linear_4bit(x, q, off), F.linear_4bit(x, q, want))
+    assert torch.equal(F.R.expert_linear(x, w, wide), F.R.expert_linear(x, w, want))
