@@ -743,7 +743,9 @@ int eri_linear_4bit(const void* x, long long ldx, const void* codes, const float
 // range's dy fits shared memory.
 int eri_linear_4bit_planes(int R, int N, int K, int block, int grouped) {
   const int cols = kU * (block % 64 == 0 ? 64 : 32), blocks = ((K + cols - 1) / cols) * (grouped ? (R + 1) / 2 : (R + kRows - 1) / kRows);
-  int s = 148 / blocks;
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) dev = 0;
+  int s = num_sms(dev) / blocks;
   const int most = (N + 16 * kDgWarps - 1) / (16 * kDgWarps), least = ((N + 15) / 16 + kDgRows / 16 - 1) / (kDgRows / 16);
   if (s > most) s = most;
   if (s < least) s = least;
