@@ -225,6 +225,7 @@ Tensor single_stream(const Tensor& xm, const Tensor& x, const Tensor& gate, cons
                      int64_t heads, int flags, bool act_fwd_epilogue, bool act_bwd_epilogue);
 
 // ---- expert_ops.cpp
+bool are_slices(const Tensor& whole, const std::vector<Tensor>& ts);
 std::vector<Tensor> expert_route(const Tensor& scores, const OptT& allowed, int64_t k, bool normalize);
 std::vector<Tensor> expert_plan(const Tensor& idx, int64_t experts);
 Tensor expert_dispatch(const Tensor& x, const Tensor& rows, const Tensor& offsets);

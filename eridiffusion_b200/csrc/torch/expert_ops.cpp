@@ -301,6 +301,19 @@ void check_plan(const char* what, const Tensor& rows, const Tensor& offsets) {
 Tensor int32(const Tensor& t) { return contig(t.scalar_type() == at::kInt ? t : t.clamp(0, std::numeric_limits<int>::max()).to(at::kInt)); }
 }  // namespace
 
+// Whether ts are the slices whole[0], whole[1], .. and record no gradients.
+bool are_slices(const Tensor& whole, const std::vector<Tensor>& ts) {
+  if (whole.size(0) != (int64_t)ts.size()) return false;
+  const char* at = (const char*)whole.data_ptr();
+  for (const Tensor& t : ts) {
+    if (t.data_ptr() != at || t.sizes() != whole.sizes().slice(1) || t.scalar_type() != whole.scalar_type() || !t.is_contiguous() ||
+        t.requires_grad() || t.device() != whole.device())
+      return false;
+    at += t.numel() * t.element_size();
+  }
+  return true;
+}
+
 std::vector<Tensor> expert_route(const Tensor& scores, const OptT& allowed_, int64_t k, bool normalize) {
   const Tensor allowed = contig(opt(allowed_));
   same_device("expert_route", scores, {&allowed});

@@ -56,6 +56,7 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("conv2d_trained", &conv2d_trained);
   m.def("upsample2x", &upsample2x);
   m.def("single_stream", &single_stream);
+  m.def("are_slices", &are_slices);
   m.def("expert_route", &expert_route);
   m.def("expert_plan", &expert_plan);
   m.def("expert_dispatch", &expert_dispatch);

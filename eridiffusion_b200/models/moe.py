@@ -23,6 +23,7 @@ import torch
 from torch.autograd import forward_ad
 
 from ..memory import QuantizedTensor, dequantize, quantize
+from ..ops import _native as N
 from ..ops import functional as F
 
 
@@ -50,7 +51,7 @@ class ExpertBank:
     def __init__(self, kind: QuantKind | str = QuantKind.Q8):
         self.kind = QuantKind(kind)
         self.experts: dict[int, object] = {}
-        self._stack = None              # (ids, where their entries lie, stacked weight)
+        self._stack = None              # (ids, what their entries are slices of, the stacked weight)
         self._streams = set()           # whose memory stacks are
         self._fixed = False             # a captured graph reads the entries where they lie, or they do not fit twice
 
@@ -68,7 +69,8 @@ class ExpertBank:
     def fetch_topk_bf16(self, ids):
         """[(id, bf16 weight)] for the ids that are present, in the order asked."""
         self._fix_if_captured()
-        return [(int(i), dequantize_to_bf16(self._here(self.experts[int(i)]))) for i in ids if int(i) in self.experts]
+        ids = [int(i) for i in ids if int(i) in self.experts]
+        return [(i, dequantize_to_bf16(e)) for i, e in zip(ids, self._here([self.experts[i] for i in ids]))]
 
     def _fix_if_captured(self) -> bool:
         """Whether the current stream captures; the entries then stay where they lie, for the replays."""
@@ -76,15 +78,16 @@ class ExpertBank:
         self._fixed |= captured
         return captured
 
-    def _here(self, weight):
-        """``weight``, an entry or a stack, for the current stream: memory of another stream's stack may not be given to others
+    def _here(self, weights):
+        """``weights``, entries or stacks, for the current stream: memory of another stream's stack may not be given to others
         before this stream has read it."""
-        if self._streams and _device(weight).type == "cuda":
-            stream = torch.cuda.current_stream(_device(weight))
-            if self._streams != {stream.cuda_stream}:
-                for t in (weight.data, weight.scale) if isinstance(weight, QuantizedTensor) else (weight,):
-                    t.record_stream(stream)
-        return weight
+        if self._streams and weights and _device(weights[0]).type == "cuda":
+            device = _device(weights[0])
+            if self._streams != {_stream(device)}:
+                for w in weights:
+                    for t in (w.data, w.scale) if isinstance(w, QuantizedTensor) else (w,):
+                        t.record_stream(torch.cuda.current_stream(device))
+        return weights
 
     def stacked(self, ids):
         """The weights of the present experts ``ids`` as one [len(ids), N, K] tensor or, for 4-bit codes, one ``QuantizedTensor`` of
@@ -96,11 +99,11 @@ class ExpertBank:
         bf16, int4 or NF4."""
         with _MOVING:
             weight = self._stacked(tuple(ids))
-        return None if weight is None else self._here(weight)
+        return None if weight is None else self._here([weight])[0]
 
     def _stacked(self, ids):
         entries = [self.experts[i] for i in ids]
-        if self._stack is not None and self._stack[0] == ids and self._stack[1] == _places(entries):
+        if self._stack is not None and self._stack[0] == ids and _lie_in(self._stack[1], self._stack[2], entries):
             return self._stack[2]
         if self._fix_if_captured() or self._fixed:
             return None
@@ -117,21 +120,24 @@ class ExpertBank:
         if joined[0].is_cuda:
             # every stream finds the stack filled, and nothing reads the old memory any more when it is given back
             torch.cuda.synchronize(joined[0].device)
-            self._streams.add(torch.cuda.current_stream(joined[0].device).cuda_stream)
+            self._streams.add(_stream(joined[0].device))
         for whole, part in zip(joined, parts):
             for t, home in zip(part, whole):
                 t.data = home
         first, weight = entries[0], joined[0]
         if isinstance(first, QuantizedTensor):
             weight = QuantizedTensor(first.kind, joined[0].flatten(0, 1), joined[1].flatten(), (len(ids), *first.shape), first.block)
-        self._stack = (ids, _places(entries), weight)
+        self._stack = (ids, joined, weight)
         return weight
 
 
-def _places(entries):
-    """What tells whether entries still lie where a stack that is alive has them."""
-    return [(e.kind, e.block, tuple(e.shape), e.data.data_ptr(), e.data.shape, e.scale.data_ptr(), e.scale.shape)
-            if isinstance(e, QuantizedTensor) else (e.data_ptr(), e.shape, e.stride(), e.dtype, e.requires_grad) for e in entries]
+def _lie_in(joined, weight, entries) -> bool:
+    """Whether the entries still are the slices of their stack."""
+    if not isinstance(weight, QuantizedTensor):
+        return not any(isinstance(e, QuantizedTensor) for e in entries) and N.ops().are_slices(joined[0], entries)
+    like = (weight.kind, tuple(weight.shape[1:]), weight.block)
+    return all(isinstance(e, QuantizedTensor) and (e.kind, tuple(e.shape), e.block) == like for e in entries) \
+        and N.ops().are_slices(joined[0], [e.data for e in entries]) and N.ops().are_slices(joined[1], [e.scale for e in entries])
 
 
 def _holders(t):
@@ -243,7 +249,7 @@ def _moe_grouped(x, idx, w, total: int, bank: ExpertBank, resident):
         if not captured:
             used = set(idx.flatten().tolist())
             ids = [i for i in ids if i in used]
-        entries = [bank._here(bank.experts[i]) for i in ids]
+        entries = bank._here([bank.experts[i] for i in ids])
         if not ids or any(tuple(e.shape) != tuple(first.shape) for e in entries):
             return None
     if any(_device(e) != x.device for e in entries or (weight,)):
@@ -272,8 +278,14 @@ def _moe_grouped(x, idx, w, total: int, bank: ExpertBank, resident):
 def _capturing(device) -> bool:
     if device is None or device.type != "cuda":
         return False
+    if device.index == torch.cuda.current_device():
+        return torch.cuda.is_current_stream_capturing()
     with torch.cuda.device(device):
         return torch.cuda.is_current_stream_capturing()
+
+
+def _stream(device) -> int:
+    return torch.cuda.current_stream(device).cuda_stream if N._raw_stream is None else N._raw_stream(device.index)
 
 
 def _device(weight):

@@ -160,6 +160,7 @@ def test_memory_of_another_streams_stack_is_recorded(monkeypatch):
     monkeypatch.setattr(torch, "stack", lambda ts: torch.cat([t[None] for t in ts]).as_subclass(OnGpu))
     monkeypatch.setattr(torch.cuda, "synchronize", lambda d: synced.append([bank.experts[i].data_ptr() for i in range(2)]))
     monkeypatch.setattr(torch.cuda, "current_stream", lambda d=None: SimpleNamespace(cuda_stream=now[0]))
+    monkeypatch.setattr(moe, "_stream", lambda d: now[0])
     monkeypatch.setattr(moe, "_device", lambda w: device)
     monkeypatch.setattr(moe, "_capturing", lambda d: False)
     before = [bank.experts[i].data_ptr() for i in range(2)]
