@@ -111,16 +111,17 @@ struct ExpertDispatch : torch::autograd::Function<ExpertDispatch> {
 };
 
 struct ExpertCombine : torch::autograd::Function<ExpertCombine> {
-  // dy and dw in operations that have gradients; choices of nobody go to a row of their own behind the others.
+  // dy and dw in operations that have gradients; choices without a row go to one of their own behind the others.
+  static Tensor nobody(const Tensor& rows) { return (rows < 0).logical_or(rows >= rows.numel()); }
   static Tensor gradient_rows(const Tensor& dout, const Tensor& w, const Tensor& rows) {
     const int64_t n = rows.numel(), D = dout.size(1);
     const Tensor dy = (w.unsqueeze(-1) * dout.to(at::kFloat).unsqueeze(1)).to(dout.scalar_type()).reshape({n, D});
-    const Tensor to = rows.masked_fill(rows < 0, n).flatten().to(at::kLong);
+    const Tensor to = rows.masked_fill(nobody(rows), n).flatten().to(at::kLong);
     return at::zeros({n + 1, D}, dout.options()).index_copy(0, to, dy).narrow(0, 0, n);
   }
   static Tensor gradient_weights(const Tensor& dout, const Tensor& y, const Tensor& rows) {
-    const Tensor yt = y.index_select(0, rows.clamp_min(0).flatten()).view({rows.size(0), rows.size(1), y.size(1)}).to(at::kFloat);
-    return (dout.to(at::kFloat).unsqueeze(1) * yt.masked_fill((rows < 0).unsqueeze(-1), 0.f)).sum(-1);
+    const Tensor yt = y.index_select(0, rows.masked_fill(nobody(rows), 0).flatten()).view({rows.size(0), rows.size(1), y.size(1)}).to(at::kFloat);
+    return (dout.to(at::kFloat).unsqueeze(1) * yt.masked_fill(nobody(rows).unsqueeze(-1), 0.f)).sum(-1);
   }
   static Tensor forward(AutogradContext* ctx, const Tensor& y, const Tensor& w, const Tensor& rows, const Tensor& offsets) {
     const CUDAGuard guard(y.device());

@@ -253,15 +253,21 @@ def expert_plan(idx, num_experts):
 
 def expert_dispatch(x, rows):
     T, k = rows.shape
-    here = rows.reshape(-1) >= 0
+    here = _placed(rows).reshape(-1)
     token = torch.arange(T, device=x.device).repeat_interleave(k)[here]
     out = x.new_zeros(T * k, x.shape[1], dtype=torch.float32)
     return out.index_copy(0, rows.reshape(-1)[here].long(), x.float()[token]).to(x.dtype)
 
 
 def expert_combine(y, w, rows):
-    yt = torch.where((rows >= 0)[..., None], y.float()[rows.clamp_min(0).long()], 0.0)
+    here = _placed(rows)
+    yt = torch.where(here[..., None], y.float()[torch.where(here, rows, 0).long()], 0.0)
     return (w.float()[..., None] * yt).sum(1).to(y.dtype)
+
+
+def _placed(rows):
+    """Choices that have a row; whatever else a plan holds is nobody's."""
+    return (rows >= 0) & (rows < rows.numel())
 
 
 def _segments(offsets, rows):

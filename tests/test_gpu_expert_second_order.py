@@ -163,3 +163,25 @@ def test_only_what_a_gradient_needs_is_kept(trained):
     assert (x.data_ptr() in kept) == (1 in pick) and (y.data_ptr() in kept) == (1 in pick)
     got = [*torch.autograd.grad(a, [(x, w)[i] for i in pick], dx), *torch.autograd.grad(b, [(y, f)[i] for i in pick], dout)]
     assert all(torch.equal(p, q) for p, q in zip(got, [want[i] for i in pick] + [want[2 + i] for i in pick]))
+
+
+def test_rows_outside_a_plan_are_nobodys():
+    """The kernels and the recorded backward pass leave them out alike."""
+    g = torch.Generator(device="cuda").manual_seed(9)
+    plan = F.expert_plan(torch.tensor([[0, 1], [1, 0], [2, 2]], device="cuda"), 3)
+    bad = plan._replace(rows=plan.rows.clone())
+    bad.rows[0, 1], bad.rows[1, 0], bad.rows[2, 1] = 6, 2 ** 31 - 1, -7
+    good = plan._replace(rows=torch.where(bad.rows < 6, bad.rows, -1).clamp_min(-1))
+    y, w, x = _mk(g, 6, 64), torch.rand(3, 2, device="cuda", generator=g), _mk(g, 3, 64)
+    dy, dx = _mk(g, 3, 64), _mk(g, 6, 64)
+    for create in (False, True):
+        got = []
+        for p in (bad, good):
+            ys, ws, xs = (t.clone().requires_grad_() for t in (y, w, x))
+            out, rows = F.expert_combine(ys, ws, p), F.expert_dispatch(xs, p)
+            here = (p.rows >= 0) & (p.rows < 6)
+            a = torch.autograd.grad(out, (ys, ws), dy, create_graph=create)
+            # a row of nobody is not written: compare the others
+            used = torch.zeros(6, dtype=torch.bool, device="cuda").index_fill(0, p.rows[here].long(), True)
+            got.append((out.detach(), a[0].detach()[used], a[1].detach(), rows.detach()[used], torch.autograd.grad(rows, xs, dx, create_graph=create)[0].detach()))
+        assert all(torch.equal(p, q) for p, q in zip(*got))
