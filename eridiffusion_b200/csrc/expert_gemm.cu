@@ -528,6 +528,11 @@ int eri_expert_gemm(int mode, const void* rows, long long ld_rows, const void* r
     // experts, 4096 x 2048 (first row 5120 x 2560):  32 | 64 | 128 | 256 columns
     //   4 rows    64.5/68.8 | 66.3/70.9 | 68.0/72.5 | 70.4/73.6       64 rows   61.0/65.0 | 53.0/50.9 | 48.9/46.7 | 51.1/47.0
     //   32 rows   47.2/50.4 | 48.1/46.0 | 47.5/45.4 | 49.7/45.4       128 rows  97.3/95.2 | 67.9/69.9 | 57.6/55.5 | 54.9/52.0
+    // Other banks, L2 flushed, 64 | 128 | 256 columns:  64 experts of 1408 x 2048    128 of 768 x 2048          4 of 8192 x 2048
+    //   32 rows                                         84/82 | 84/78 | 86/78        90/88 | 90/86 | 92/84      37/39 | 37/43 | 39/47
+    //   128 rows                                        100/100 | 88/86 | 94/84      107/121 | 96/100 | 102/94  43/41 | 43/45 | 41/53
+    //   512 rows                                        285/281 | 184/180 | 158/152  (256) 166/193 | 129/137 | 115/119  100/105 | 68/72 | 66/94
+    // The rule is within a tenth of the best of the three but for dX of four experts of 8192 x 2048 (few, wide tiles: 53 for 41, 94 for 72).
     const int per = R / E;
     bt = per <= 8 ? 32 : per <= 16 ? 64 : per <= 96 ? 128 : 256;
   }

@@ -220,8 +220,8 @@ def dequantize(q: QuantizedTensor, dtype=torch.bfloat16, out=None):
 
 class QuantizedLinear(nn.Module):
     """Frozen base weight stored quantised; dequantised per call into a scratch tensor and fed to
-    the fused linear (adapters attach as usual). A few rows on a 4-bit weight without adapter (conditioning
-    vectors) are multiplied with the codes themselves."""
+    the fused linear (adapters attach as usual). A few bf16 rows on a 4-bit weight without adapter are multiplied
+    with the codes themselves."""
 
     def __init__(self, linear, kind="int8", block=64):
         super().__init__()

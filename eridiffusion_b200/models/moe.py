@@ -6,7 +6,10 @@ moe_quant.rs:6-48). In the reference the quantiser is a pass-through and the sel
 first k ids. Here the bank stores real int8 / NF4 codes (``memory.quantize``; expanded by the
 dequantisation kernel on the GPU) and the selection is a top-k over router scores. On the GPU the tokens
 are put into expert order (``F.expert_plan`` / ``expert_dispatch``), meet all experts in one grouped product
-(``F.expert_linear``, or ``F.linear_4bit`` on the codes of a 4-bit bank) and are added up again (``F.expert_combine``).
+(``F.expert_linear``, or ``F.linear_4bit`` on the codes of a 4-bit bank and few rows) and are added up again
+(``F.expert_combine``). Nothing is read back where the bank's weights can be stacked (``ExpertBank.stacked``) and all experts are
+resident; int8 codes, 4-bit codes of many rows and weights that someone else holds are expanded or joined for each call, only
+the experts that some token uses, which are read back.
 
 Wan 2.2 itself is not token-routed: its two "experts" are two whole transformers chosen by the
 timestep (``models/nextdit.py``: ``WanDualExpert``); the bank serves that case too (two entries,

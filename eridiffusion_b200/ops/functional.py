@@ -1040,7 +1040,15 @@ def expert_linear(x, w, offsets):
 
 
 # Most rows that are multiplied with the codes themselves; above, the weight is expanded once and meets the matrix kernels. Widest row:
-# x of a pass, the rings and the tables share an SM's memory.
+# x of a pass, the rings and the tables share an SM's memory. us on the codes | expanded, product alone and with the rows' gradient:
+#   rows of a weight        8                  9                  16                 32                  64
+#   NF4 15360 x 2560        17 | 35, 38 | 50   26 | 35, 75 | 56   28 | 35, 78 | 50   45 | 35, 119 | 50   81 | 35, 201 | 56
+#   int4 13824 x 5120       21 | 63, 49 | 87   27 | 66, 80 | 92   27 | 66, 80 | 89   46 | 66, 149 | 89   86 | 68, 286 | 98
+#   NF4 2560 x 2560          8 | 14, 19 | 21   11 | 12, 23 | 18   11 | 12, 24 | 18   14 | 12, 31 | 18    20 | 12, 57 | 18
+# so eight rows win in both directions everywhere; without a gradient 16 to 48 rows would, too. Experts (16 rows, 64, 128; all experts
+# have rows, where nothing is read for an empty one the codes win by more):
+#   NF4 16 of 5120 x 2560   48 | 194, 138 | 271   48 | 194, 145 | 270   52 | 194, 156 | 270
+#   int4 8 of 2048 x 2048   12 | 34, 30 | 45      13 | 34, 44 | 46      20 | 34, 55 | 46
 CODES_ROWS, CODES_EXPERT_ROWS, _CODES_WIDTH = 8, 64, 16384
 
 

@@ -223,3 +223,24 @@ def test_router_under_transforms():
         assert torch.equal(idx[b], i1) and torch.allclose(w[b], w1, atol=1e-6)
     _, dw = torch.func.jvp(lambda t: route_tokens(t, 2)[1], (s[0],), (torch.ones_like(s[0]),))
     assert dw.abs().max().item() < 1e-6           # weights do not change when all scores grow alike
+
+
+@pytest.mark.parametrize("T", [1, 5, 30, 400])
+@pytest.mark.parametrize("kind", ["none", "q8", "nf4"])
+def test_against_the_weights_that_are_multiplied(kind, T):
+    """Expanded weights are bf16 as they are; codes on few rows are levels in 11 bits times their scale. What is left are the roundings of
+    the chosen experts' outputs and of their sum (2^-8 of themselves each) and sums over K in 32 bits."""
+    from eridiffusion_b200.ops import functional as F
+    g = torch.Generator(device="cuda").manual_seed(T + 20)
+    bank = _bank(kind, g)
+    x, scores = _inputs(g, T)
+    on_codes = kind == "nf4" and 2 * T <= F.CODES_EXPERT_ROWS
+    ws = torch.stack([_weight64(e) if kind == "none" or on_codes else e.dequantize(BF).double() for e in bank.experts.values()])
+    top, idx = torch.sort(scores.double(), dim=-1, descending=True, stable=True)
+    w, xd = torch.softmax(top[:, :2], -1), x.double()
+    ref = torch.einsum("tjnk,tk->tjn", ws[idx[:, :2]], xd)
+    mag = torch.einsum("tjnk,tk->tjn", ws[idx[:, :2]].abs(), xd.abs())
+    err = (w[..., None] * (ref.abs() * 2 ** -8 + mag * (K * 2 ** -23 + (2 ** -11 if on_codes else 0)))).sum(1)
+    ref = (w[..., None] * ref).sum(1)
+    y = moe_linear(x, scores, bank)
+    assert ((y.double() - ref).abs() <= (ref.abs() * 2 ** -8 + err) * 1.01 + 1e-30).all()
