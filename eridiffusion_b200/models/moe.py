@@ -258,6 +258,8 @@ def _moe_grouped(x, idx, w, total: int, bank: ExpertBank, resident):
     if any(_device(e) != x.device for e in entries or (weight,)):
         return None
     if len(ids) != total:                    # the experts' places in the bank; an absent expert adds nothing
+        if captured:
+            raise RuntimeError("moe_linear: a bank with absent experts cannot be captured (their places are copied from the host)")
         place = torch.full((total,), -1, dtype=torch.int64)
         place[ids] = torch.arange(len(ids))
         idx = place.to(x.device)[idx]

@@ -244,3 +244,20 @@ def test_against_the_weights_that_are_multiplied(kind, T):
     ref = (w[..., None] * ref).sum(1)
     y = moe_linear(x, scores, bank)
     assert ((y.double() - ref).abs() <= (ref.abs() * 2 ** -8 + err) * 1.01 + 1e-30).all()
+
+
+@pytest.mark.parametrize("what", ["absent", "resident"])
+def test_captures_that_need_the_host_are_refused(what):
+    g = torch.Generator(device="cuda").manual_seed(30)
+    bank = _bank("none", g)
+    x, scores = _inputs(g, 5)
+    if what == "absent":
+        del bank.experts[2]
+    graph = torch.cuda.CUDAGraph()
+    with pytest.raises(RuntimeError):
+        with torch.cuda.graph(graph):
+            moe_linear(x, scores, bank, resident=3 if what == "resident" else None)
+    torch.cuda.synchronize()
+    y = moe_linear(x, scores, bank)
+    if what == "resident":
+        _near(y, x, scores, bank)
