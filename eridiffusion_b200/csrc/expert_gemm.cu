@@ -532,7 +532,8 @@ int eri_expert_gemm(int mode, const void* rows, long long ld_rows, const void* r
     //   32 rows                                         84/82 | 84/78 | 86/78        90/88 | 90/86 | 92/84      37/39 | 37/43 | 39/47
     //   128 rows                                        100/100 | 88/86 | 94/84      107/121 | 96/100 | 102/94  43/41 | 43/45 | 41/53
     //   512 rows                                        285/281 | 184/180 | 158/152  (256) 166/193 | 129/137 | 115/119  100/105 | 68/72 | 66/94
-    // The rule is within a tenth of the best of the three but for dX of four experts of 8192 x 2048 (few, wide tiles: 53 for 41, 94 for 72).
+    // The rule is within a tenth of the best but for dX of few experts, whose tiles do not fill the pairs evenly: four of 8192 x 2048
+    // 53 where 41 is possible (128 rows) and 94 for 72 (512), eight of 5120 x 2560 62 for 53 (64 rows) and 72 for 57 (128).
     const int per = R / E;
     bt = per <= 8 ? 32 : per <= 16 ? 64 : per <= 96 ? 128 : 256;
   }
