@@ -439,7 +439,8 @@ __global__ void __launch_bounds__(kMaxWarps * 32, 1) linear_4bit_kernel(const Ar
 // 2^-22 of the largest keep all their bits, the rest is off by 2^-33 of it.
 // A CTA owns one piece of columns (256, or 128 with blocks of 32) and a range of weight rows; its warps take every kDgWarps-th 16 rows, their
 // sums meet in shared memory in warp order, and the ranges' planes are added in order by the kernel below. us: 13824 x 5120 int4, eight
-// rows, 22 and 4 for the planes (160 with one thread per eight columns and the products in 32 bits).
+// rows, 22 and 4 for the planes (160 with one thread per eight columns and the products in 32 bits); 16 rows over 16 NF4 experts of 5120 x 2560,
+// 90.
 constexpr int kDgWarps = 16, kDgDepth = 3, kDgRows = 2048;        // kDgRows: most weight rows of a range (their dy is in shared memory)
 
 template <bool NF4>
